@@ -333,8 +333,8 @@ def _append(s):
     P = c["page"]
     if own:
         from vkcuda_b200 import vc
-        vc.check(vc.kv8_append(s["cache"], s["kn"], s["vn"], s["table"], s["table"].shape[1], s["start"],
-                               c["B"], s["most"],
+        vc.check(vc.kv8_append(s["cache"], s["kn"], s["vn"], s["tokens"], s["table"],
+                               s["table"].shape[1], s["start"], c["B"], s["most"],
                                vc.Dtype.F16 if c["dtype"] == "fp16" else vc.Dtype.BF16,
                                cu=s["cu"], lens_out=s["lens"]), "kv8_append")
         return [s["k"], s["v"], s["ks"], s["vs"], s["lens"]]
