@@ -13,6 +13,9 @@
  *     They replace the bodies of the demo kernels named on each
  *     (examples/flash_attn.vc, test/wmma_gemm.vc,
  *     examples/matmul_coopmat_bench.vc, test/vadd.vc, test/reduce.vc).
+ *     Behind them the serving entries (no counterpart in the reference):
+ *     prompt attention through a sliding window, and an 8-bit paged K/V cache
+ *     with its append, single-token attention, page copy and page pool.
  *
  * Pointers passed to kernels are device addresses (vc_malloc, cudaMalloc or a
  * torch tensor's data_ptr). `stream` is a CUDA stream handle (cudaStream_t);
@@ -251,6 +254,118 @@ int vc_gemm(const void *A, const void *B, float *D, const float *Cin, int M,
 int vc_flash_fwd(const void *Q, const void *K, const void *V, void *O, int BH,
                  int N, int d, float scale_log2, int causal, int dtype,
                  void *stream);
+
+/* ---- Serving entries. Beside the usual errors they refuse, with
+ * VC_INVALID_VALUE and before any launch, a pointer that this device cannot
+ * read (host memory, another device's). With `stream` NULL they join a graph
+ * that is being recorded (vc_graph_begin_record), as vc_launch_kernel does.
+ * What lies in device memory (lengths, offsets, page numbers) is checked by
+ * the kernels: what is out of range is left out and vc_kernel_error reports
+ * it (4, out of bounds). */
+
+/* Causal flash attention of prompts through a sliding window, with a few first
+ * tokens that stay visible (sinks). Query row i of a sequence stands at
+ * position t = i + Nk - Nq (Nk > Nq: a later chunk of a prompt) and sees the
+ * keys j <= t with t - j < window or j < sinks; window 0: every j <= t.
+ *   O[b][h][i] = sum_j p_j V[b][h / (Hq / Hkv)][j],
+ *   p = softmax_2(scale_log2 * Q[b][h][i] . K[b][h / (Hq / Hkv)][j]).
+ * A row that sees no key (t < 0) is zero. Hq is a multiple of Hkv, d 64 or
+ * 128, dtype F16 or BF16. The strides (elements between batches, heads and
+ * tokens, in this order; NULL: dense [B][H][N][d]) are multiples of 8, rows
+ * contiguous and 16-byte aligned; along an axis of one entry they do not
+ * matter. `lens` (optional, device, B entries): sequence b has lens[b] tokens
+ * (clamped to [0, Nk]); what K and V hold behind them is not used, whatever it
+ * is, and rows of O at positions t >= lens[b] are left as they were. V of a
+ * sequence's own tokens has to be finite, as for vc_flash_fwd. */
+int vc_flash_window_fwd(const void *Q, const void *K, const void *V, void *O, int B, int Hq,
+                        int Hkv, int Nq, int Nk, int d, const int64_t *q_strides,
+                        const int64_t *k_strides, const int64_t *v_strides,
+                        const int64_t *o_strides, const int32_t *lens, int window, int sinks,
+                        float scale_log2, int dtype, void *stream);
+
+/* One layer of a paged K/V cache held in 8 bits. A page holds `page_size`
+ * tokens (16, 32, 64 or 128) of every K/V head: codes [heads][page_size]
+ * [head_dim] in e4m3, and one fp32 scale for each head, K and V apart; a code
+ * stands for code * scale. Page i's codes start page_stride bytes (a multiple
+ * of 16) behind page i - 1's, its scales scale_stride floats; k and v are
+ * 16-byte aligned; head_dim is 64 or 128. Layers may share one allocation. */
+typedef struct vc_kv8_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int num_pages, heads, page_size, head_dim;
+  int64_t page_stride;  /* >= heads * page_size * head_dim */
+  int64_t scale_stride; /* >= heads */
+} vc_kv8_cache;
+
+/* Append: sequence b's new tokens (rows cu[b] .. cu[b + 1] of K and V, at most
+ * max_new; cu NULL: max_new rows each) to its slots start[b], start[b] + 1, ...
+ * Slot s lies in page table[b * table_width + s / page_size]. K and V are
+ * [tokens][heads][head_dim], F16 or BF16, k_stride / v_stride elements between
+ * tokens (multiples of 8, rows 16-byte aligned). A page's scale is the power
+ * of two 2^e with the smallest e (-100 <= e <= 119) that holds the largest
+ * finite new magnitude within 448 * 2^e, or the scale that it has if that is
+ * larger and the page holds earlier tokens of the sequence; when it grows,
+ * those are re-expressed. Values round to nearest even; infinities become the
+ * largest code, NaN stays NaN. Slots behind the new tokens are left as they
+ * were. A page that takes tokens belongs to one sequence (see
+ * vc_kv8_pool_extend). lens_out (optional, B entries, not `start` itself)
+ * receives start[b] + the tokens added. */
+int vc_kv8_append(const vc_kv8_cache *cache, const void *K, const void *V, int64_t k_stride,
+                  int64_t v_stride, int tokens, const int32_t *table, int table_width,
+                  const int32_t *start, const int32_t *cu, int B, int max_new,
+                  int32_t *lens_out, int dtype, void *stream);
+
+/* Attention of one token for each sequence over the cache: Q and O are
+ * [B][Hq][head_dim] (q_stride / o_stride elements between sequences, multiples
+ * of 8, 16-byte aligned), F16 or BF16. The token of sequence b is its last,
+ * at position lens[b] - 1, and sees the keys j < lens[b] with
+ * j >= lens[b] - window (window 0: all) or j < sinks. lens[b] = 0 gives a zero
+ * row. Hq is a multiple of cache->heads. Any positive scales within 2^-100 ..
+ * 2^119 (and 0) are taken. Several tokens of one sequence (a draft to verify)
+ * are several rows with the same pages and growing lens.
+ * workspace: vc_kv8_attn_workspace bytes, 256-byte aligned, zero before its
+ * first call and left ready for the next, of whatever shape; calls that may
+ * overlap (two streams, two graphs) need one each. */
+int vc_kv8_attn_workspace(const vc_kv8_cache *cache, int B, int Hq, size_t *bytes);
+int vc_kv8_attn(const vc_kv8_cache *cache, const void *Q, int64_t q_stride, void *O,
+                int64_t o_stride, const int32_t *table, int table_width, const int32_t *lens,
+                int B, int Hq, int window, int sinks, float scale_log2, int dtype,
+                void *workspace, size_t workspace_bytes, void *stream);
+
+/* Copy pages src[i] -> dst[i], i < n (device arrays), codes and scales, in all
+ * n_layers layers (a host array; same num_pages, heads, page_size, head_dim
+ * and strides). No page may be the target of two copies, nor the target of one
+ * and the source of another. */
+int vc_kv8_copy_pages(const vc_kv8_cache *layers, int n_layers, const int32_t *src,
+                      const int32_t *dst, int n, void *stream);
+
+/* The pool: which pages belong to which sequence (host bookkeeping, no GPU;
+ * calls may come from several threads). Free pages are handed out lowest
+ * first. A call that fails changes nothing. */
+int vc_kv8_pool_create(void **pool, int num_pages, int page_size);
+int vc_kv8_pool_destroy(void *pool);
+int vc_kv8_pool_new(void *pool, int64_t *seq);  /* an empty sequence */
+/* A sequence with the same tokens, on the same pages. */
+int vc_kv8_pool_fork(void *pool, int64_t seq, int64_t *child);
+/* Room for `tokens` more: VC_OUT_OF_MEMORY when the free pages do not hold
+ * them. When the first of them falls into a page that another sequence holds
+ * too, the sequence gets a page of its own for it: copy_src -> copy_dst then
+ * say which page to copy (vc_kv8_copy_pages) before the append, else both are
+ * -1. */
+int vc_kv8_pool_extend(void *pool, int64_t seq, int64_t tokens, int32_t *copy_src,
+                       int32_t *copy_dst);
+/* Frees a sequence; pages that no other holds are free again. */
+int vc_kv8_pool_free(void *pool, int64_t seq);
+/* A sequence's pages in order, -1 behind them up to `capacity` (a row of the
+ * page table), and its counts; pages NULL: the counts alone. */
+int vc_kv8_pool_pages(void *pool, int64_t seq, int32_t *pages, int capacity, int *n_pages,
+                      int64_t *n_tokens);
+int vc_kv8_pool_info(void *pool, int *free_pages, int *sequences);
+/* Moves the held pages to the lowest numbers: copies to make, in
+ * copy_src -> copy_dst (no page is in both); the tables change with this call.
+ * More than `capacity` moves: VC_INVALID_VALUE and *n_copies says how many. */
+int vc_kv8_pool_compact(void *pool, int32_t *copy_src, int32_t *copy_dst, int capacity,
+                        int *n_copies);
 
 #ifdef __cplusplus
 }

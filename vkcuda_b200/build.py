@@ -34,6 +34,10 @@ SOURCES = [
     "gemm_simt.cu",
     "flash_fwd_tcgen05.cu",
     "flash_fwd_f32.cu",
+    "flash_window.cu",
+    "kv8_pages.cu",
+    "kv8_attn.cu",
+    "kv8_pool.cpp",
     "selftest.cu",
 ]
 

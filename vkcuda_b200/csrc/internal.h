@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 
+#include "../../include/vc_b200.h"
+
 namespace vcb {
 
 // ---- streaming (stream_kernels.cu)
@@ -104,12 +106,62 @@ struct FlashArgs {
 cudaError_t launch_flash_fwd_tcgen05(const FlashArgs &f, cudaStream_t stream);
 cudaError_t launch_flash_fwd_f32(const FlashArgs &f, cudaStream_t stream);
 
+// ---- windowed prompt attention (flash_window.cu). Strides in elements:
+// batch, head, token.
+struct FlashWindowArgs {
+  const void *Q, *K, *V;
+  void *O;
+  int B, Hq, Hkv, Nq, Nk, d;
+  int64_t sq[3], sk[3], sv[3], so[3];
+  const int32_t *lens;  // optional
+  int window, sinks;    // window 0: none
+  float scale_log2;
+  int dtype;
+};
+cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream);
+
+// ---- 8-bit paged K/V cache (kv8_pages.cu, kv8_attn.cu)
+struct Kv8AppendArgs {
+  const vc_kv8_cache *cache;
+  const void *K, *V;
+  int64_t k_stride, v_stride;
+  int T;
+  const int32_t *table;
+  int table_width;
+  const int32_t *start, *cu;
+  int B, max_new;
+  int32_t *lens_out;
+  int dtype;
+};
+cudaError_t launch_kv8_append(const Kv8AppendArgs &a, cudaStream_t stream);
+cudaError_t launch_kv8_copy(const vc_kv8_cache *layers, int n_layers, const int32_t *src,
+                            const int32_t *dst, int n, cudaStream_t stream);
+struct Kv8AttnArgs {
+  const vc_kv8_cache *cache;
+  const void *Q;
+  int64_t q_stride;
+  void *O;
+  int64_t o_stride;
+  const int32_t *table;
+  int table_width;
+  const int32_t *lens;
+  int B, Hq, window, sinks;
+  float scale_log2;
+  int dtype;
+  void *workspace;
+};
+size_t kv8_attn_workspace_bytes(const vc_kv8_cache &c, int B, int Hq);
+cudaError_t launch_kv8_attn(const Kv8AttnArgs &a, cudaStream_t stream);
+
 // ---- device error words, one accessor per translation unit
 int stream_kernels_error(int clear);
 int gemm_tcgen05_error(int clear);
 int gemm_f32_error(int clear);
 int flash_tcgen05_error(int clear);
 int selftest_error(int clear);
+int flash_window_error(int clear);
+int kv8_pages_error(int clear);
+int kv8_attn_error(int clear);
 cudaError_t launch_selftest_bounded_wait(unsigned timeout_us, cudaStream_t stream);
 
 // ---- runtime-owned scratch (runtime.cpp): per (device, stream) partials

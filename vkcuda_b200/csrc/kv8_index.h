@@ -1,0 +1,85 @@
+// kv8_index.h - index arithmetic of the 8-bit paged K/V cache, shared by its
+// kernels and (compiled as plain C++) by the CPU tests: which keys a token
+// sees, in which tiles they lie, how the tiles of a ragged batch are split
+// over blocks, and the exponent of a block's scale.
+#pragma once
+#include <cstdint>
+#include <cstring>
+
+#ifdef __CUDACC__
+#define VCB_HD __host__ __device__ __forceinline__
+#else
+#define VCB_HD inline
+#endif
+
+namespace vcb {
+
+// Keys that the last token of a sequence of `len` tokens sees: [0, sink) and
+// [lo, len), sink <= lo. window <= 0: all of them (sink = lo = 0).
+struct VisibleKeys {
+  int sink, lo, len;
+};
+VCB_HD VisibleKeys visible_keys(int len, int window, int sinks) {
+  VisibleKeys v{0, 0, len > 0 ? len : 0};
+  if (window > 0 && window < v.len) {
+    v.lo = v.len - window;
+    v.sink = sinks < v.lo ? sinks : v.lo;
+  }
+  return v;
+}
+VCB_HD bool key_visible(const VisibleKeys &v, int key) {
+  return key < v.len && (key >= v.lo || key < v.sink);
+}
+
+// Those keys as tiles of `tile` keys aligned to multiples of `tile`: first
+// `head` tiles from key 0 (the sinks), then the window's from tile `first`.
+struct VisibleTiles {
+  int head, first, count;
+};
+VCB_HD VisibleTiles visible_tiles(const VisibleKeys &v, int tile) {
+  VisibleTiles t;
+  t.first = v.lo / tile;
+  const int end = (int)(((int64_t)v.len + tile - 1) / tile);
+  t.head = (v.sink + tile - 1) / tile;
+  if (t.head > t.first) t.head = t.first;  // the window's first tile holds the rest
+  t.count = t.head + end - t.first;
+  return t;
+}
+// First key of tile `i` (0 <= i < count).
+VCB_HD int tile_key(const VisibleTiles &t, int i, int tile) {
+  return (i < t.head ? i : t.first + (i - t.head)) * tile;
+}
+
+// Split of `total` tiles over `blocks` blocks: block c takes [start(c), start(c + 1)).
+VCB_HD int64_t split_start(int64_t total, int blocks, int c) { return total * c / blocks; }
+// The block that takes tile t: the largest c with start(c) <= t.
+VCB_HD int split_owner(int64_t total, int blocks, int64_t t) {
+  return (int)(((t + 1) * blocks + total - 1) / total - 1);
+}
+
+// Scale of a block whose largest finite magnitude is `amax`: 2^e, e the
+// smallest exponent with amax <= 448 * 2^e (448: the largest e4m3 value,
+// 1.75 * 2^8), kept within [-100, 119]. A power of two makes x / scale exact,
+// so that the only rounding is the one to 8 bits, and tokens whose scale
+// grows later move without a second rounding but in e4m3's subnormals.
+constexpr int kScaleMinExp = -100, kScaleMaxExp = 119;
+VCB_HD float e4m3_block_scale(float amax) {
+  uint32_t b;
+#ifdef __CUDA_ARCH__
+  b = __float_as_uint(amax);
+#else
+  std::memcpy(&b, &amax, 4);
+#endif
+  int e = (int)((b >> 23) & 0xFFu) - 127 - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  e = e < kScaleMinExp ? kScaleMinExp : e > kScaleMaxExp ? kScaleMaxExp : e;
+  const uint32_t s = (uint32_t)(e + 127) << 23;
+#ifdef __CUDA_ARCH__
+  return __uint_as_float(s);
+#else
+  float f;
+  std::memcpy(&f, &s, 4);
+  return f;
+#endif
+}
+
+}  // namespace vcb

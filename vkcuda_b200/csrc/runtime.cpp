@@ -1457,6 +1457,285 @@ VCError k_native_flash(VCKernel &, const LaunchShape &, const VCKernelArg *a, in
   return flash_checked(f, s);
 }
 
+// ---- serving entries: prompt attention through a window, 8-bit paged cache
+
+// Whether kernels of the current device can read p: its own or managed memory,
+// or pinned host memory. (What lies behind a wrong pointer would be a GPU
+// fault, so foreign memory is asked for too.)
+bool device_readable(const void *p) {
+  cudaPointerAttributes a;
+  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (a.type == cudaMemoryTypeDevice) return a.device == t_device;
+  return a.type == cudaMemoryTypeManaged || a.type == cudaMemoryTypeHost;
+}
+// The last step before a launch, once the arguments are known to be in order
+// (which needs no GPU): the runtime is up and every pointer is readable.
+VCError ready_to_launch(const char *k, std::initializer_list<const void *> pointers) {
+  if (!ensure_init()) return VCError::InitializationError;
+  use_current_device();
+  for (const void *p : pointers)
+    if (p && !device_readable(p)) {
+      std::fprintf(stderr, "vc: kernel %s: a pointer is not memory of the current device\n", k);
+      return VCError::InvalidValue;
+    }
+  return VCError::Success;
+}
+bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Device arrays of `n` 32-bit entries.
+VCError ints_checked(const void *p, size_t n, const char *name) {
+  if (!p || !aligned(p, 4)) return VCError::InvalidValue;
+  return n * 4 > bytes_available(p) ? too_small(name) : VCError::Success;
+}
+
+// Bytes that [B][H][N][d] 16-bit elements at these strides span.
+size_t span16(int B, int H, int N, int d, const int64_t *s) {
+  return (size_t)((B - 1) * s[0] + (H - 1) * s[1] + (int64_t)(N - 1) * s[2] + d) * 2;
+}
+
+VCError flash_window_checked(vcb::FlashWindowArgs f, const int64_t *const strides[4],
+                             cudaStream_t s) {
+  const char *name = "vc.flash_window";
+  if (f.B <= 0 || f.Hq <= 0 || f.Hkv <= 0 || f.Nq <= 0 || f.Nk <= 0 || f.Hq % f.Hkv)
+    return VCError::InvalidValue;
+  if (f.dtype != VC_DTYPE_F16 && f.dtype != VC_DTYPE_BF16) return VCError::InvalidValue;
+  if ((f.d != 64 && f.d != 128) || f.window < 0 || f.sinks < 0) return VCError::InvalidValue;
+  if ((int64_t)f.B * f.Hq > 65535) return VCError::InvalidValue;
+  int64_t *const to[4] = {f.sq, f.sk, f.sv, f.so};
+  const void *const p[4] = {f.Q, f.K, f.V, f.O};
+  for (int i = 0; i < 4; ++i) {
+    const int H = i == 0 || i == 3 ? f.Hq : f.Hkv, N = i == 0 || i == 3 ? f.Nq : f.Nk;
+    const int64_t dense[3] = {(int64_t)H * N * f.d, (int64_t)N * f.d, f.d};
+    const int sizes[3] = {f.B, H, N};
+    for (int j = 0; j < 3; ++j) {
+      // Along an axis of one entry the stride is not used; a dense one keeps
+      // it within what a tensor map takes.
+      to[i][j] = strides[i] && sizes[j] > 1 ? strides[i][j] : dense[j];
+      if (to[i][j] < f.d || to[i][j] % 8 || to[i][j] >= (int64_t)1 << 38) return VCError::InvalidValue;
+    }
+    if (!p[i] || !aligned(p[i], 16)) return VCError::InvalidValue;
+    if (span16(f.B, H, N, f.d, to[i]) > bytes_available(p[i])) return too_small(name);
+  }
+  VCError e = f.lens ? ints_checked(f.lens, f.B, name) : VCError::Success;
+  if (e == VCError::Success) e = ready_to_launch(name, {f.Q, f.K, f.V, f.O, f.lens});
+  if (e != VCError::Success) return e;
+  // Dense outputs only: between strided rows lies memory that is not O's.
+  if (!f.lens && f.so[0] == (int64_t)f.Hq * f.Nq * f.d &&
+      ((f.so[1] == (int64_t)f.Nq * f.d && f.so[2] == f.d) ||
+       (f.so[1] == f.d && f.so[2] == (int64_t)f.Hq * f.d)))
+    poison_output(name, f.O, span16(f.B, f.Hq, f.Nq, f.d, f.so), s,
+                  {{f.Q, span16(f.B, f.Hq, f.Nq, f.d, f.sq)},
+                   {f.K, span16(f.B, f.Hkv, f.Nk, f.d, f.sk)},
+                   {f.V, span16(f.B, f.Hkv, f.Nk, f.d, f.sv)}});
+  return run(vcb::launch_flash_window(f, s), name);
+}
+
+VCError kv8_cache_checked(const vc_kv8_cache &c, const char *name) {
+  if (c.num_pages <= 0 || c.heads <= 0 || c.heads > 65535) return VCError::InvalidValue;
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128)
+    return VCError::InvalidValue;
+  if (c.head_dim != 64 && c.head_dim != 128) return VCError::InvalidValue;
+  const int64_t page = (int64_t)c.heads * c.page_size * c.head_dim;
+  if (page > INT32_MAX / 2 || c.page_stride < page || c.page_stride % 16 ||
+      c.page_stride > (int64_t)1 << 40 || c.scale_stride < c.heads ||
+      c.scale_stride > (int64_t)1 << 40)
+    return VCError::InvalidValue;
+  const void *const p[4] = {c.k, c.v, c.k_scale, c.v_scale};
+  for (int i = 0; i < 4; ++i) {
+    if (!p[i] || !aligned(p[i], i < 2 ? 16 : 4)) return VCError::InvalidValue;
+    const size_t need = i < 2 ? (size_t)(c.num_pages - 1) * c.page_stride + page
+                              : ((size_t)(c.num_pages - 1) * c.scale_stride + c.heads) * 4;
+    if (need > bytes_available(p[i])) return too_small(name);
+  }
+  return VCError::Success;
+}
+// Rows of `width` 16-bit elements, `stride` apart.
+VCError rows_checked(const void *p, int64_t rows, int64_t width, int64_t stride, const char *name) {
+  if (!p || !aligned(p, 16) || stride < width || stride % 8 || stride > (int64_t)1 << 38)
+    return VCError::InvalidValue;
+  if (rows <= 0) return VCError::Success;
+  return (size_t)((rows - 1) * stride + width) * 2 > bytes_available(p) ? too_small(name)
+                                                                        : VCError::Success;
+}
+
+VCError kv8_append_checked(const vcb::Kv8AppendArgs &a, cudaStream_t s) {
+  const char *name = "vc.kv8_append";
+  if (!a.cache || a.B < 0 || a.max_new < 0 || a.T < 0 || a.table_width <= 0)
+    return VCError::InvalidValue;
+  if (a.dtype != VC_DTYPE_F16 && a.dtype != VC_DTYPE_BF16) return VCError::InvalidValue;
+  if (!a.cu && (int64_t)a.B * a.max_new > a.T) return VCError::InvalidValue;
+  VCError e = kv8_cache_checked(*a.cache, name);
+  if (e != VCError::Success || a.B == 0) return e;
+  const int64_t width = (int64_t)a.cache->heads * a.cache->head_dim;
+  if ((e = rows_checked(a.K, a.T, width, a.k_stride, name)) != VCError::Success) return e;
+  if ((e = rows_checked(a.V, a.T, width, a.v_stride, name)) != VCError::Success) return e;
+  if ((e = ints_checked(a.table, (size_t)a.B * a.table_width, name)) != VCError::Success) return e;
+  if ((e = ints_checked(a.start, a.B, name)) != VCError::Success) return e;
+  if (a.cu && (e = ints_checked(a.cu, (size_t)a.B + 1, name)) != VCError::Success) return e;
+  if (a.lens_out) {
+    if ((e = ints_checked(a.lens_out, a.B, name)) != VCError::Success) return e;
+    const size_t n = (size_t)a.B * 4;
+    if (spans_overlap(a.lens_out, n, {{a.start, n}, {a.cu, a.cu ? n + 4 : 0}, {a.table, n * a.table_width}}))
+      return VCError::InvalidValue;
+  }
+  const vc_kv8_cache &c = *a.cache;
+  e = ready_to_launch(name, {c.k, c.v, c.k_scale, c.v_scale, a.K, a.V, a.table, a.start, a.cu,
+                             a.lens_out});
+  if (e != VCError::Success) return e;
+  return run(vcb::launch_kv8_append(a, s), name);
+}
+
+VCError kv8_attn_checked(const vcb::Kv8AttnArgs &a, size_t workspace_bytes, cudaStream_t s) {
+  const char *name = "vc.kv8_attn";
+  if (!a.cache || a.B < 0 || a.Hq <= 0 || a.table_width <= 0 || a.window < 0 || a.sinks < 0)
+    return VCError::InvalidValue;
+  if (a.dtype != VC_DTYPE_F16 && a.dtype != VC_DTYPE_BF16) return VCError::InvalidValue;
+  if (a.B > 65535 || a.Hq > 65535) return VCError::InvalidValue;
+  VCError e = kv8_cache_checked(*a.cache, name);
+  if (e != VCError::Success) return e;
+  const vc_kv8_cache &c = *a.cache;
+  if (a.Hq % c.heads || (int64_t)a.table_width * c.page_size > INT32_MAX) return VCError::InvalidValue;
+  if (a.B == 0) return VCError::Success;
+  const int64_t width = (int64_t)a.Hq * c.head_dim;
+  if ((e = rows_checked(a.Q, a.B, width, a.q_stride, name)) != VCError::Success) return e;
+  if ((e = rows_checked(a.O, a.B, width, a.o_stride, name)) != VCError::Success) return e;
+  if ((e = ints_checked(a.table, (size_t)a.B * a.table_width, name)) != VCError::Success) return e;
+  if ((e = ints_checked(a.lens, a.B, name)) != VCError::Success) return e;
+  if (!a.workspace || !aligned(a.workspace, 256)) return VCError::InvalidValue;
+  if (workspace_bytes > bytes_available(a.workspace)) return too_small(name);
+  e = ready_to_launch(name, {c.k, c.v, c.k_scale, c.v_scale, a.Q, a.O, a.table, a.lens, a.workspace});
+  if (e != VCError::Success) return e;
+  if (workspace_bytes < vcb::kv8_attn_workspace_bytes(c, a.B, a.Hq)) return too_small(name);
+  poison_output(name, a.O, (size_t)a.o_stride * 2, (size_t)width * 2, (size_t)a.B, s,
+                {{a.Q, (size_t)((a.B - 1) * a.q_stride + width) * 2}});
+  return run(vcb::launch_kv8_attn(a, s), name);
+}
+
+VCError kv8_copy_checked(const vc_kv8_cache *layers, int n_layers, const int32_t *src,
+                         const int32_t *dst, int n, cudaStream_t s) {
+  const char *name = "vc.kv8_copy_pages";
+  if (!layers || n_layers <= 0 || n < 0) return VCError::InvalidValue;
+  for (int i = 0; i < n_layers; ++i) {
+    const vc_kv8_cache &c = layers[i], &f = layers[0];
+    if (c.num_pages != f.num_pages || c.heads != f.heads || c.page_size != f.page_size ||
+        c.head_dim != f.head_dim || c.page_stride != f.page_stride ||
+        c.scale_stride != f.scale_stride)
+      return VCError::InvalidValue;
+    VCError e = kv8_cache_checked(c, name);
+    if (e != VCError::Success) return e;
+  }
+  if (n == 0) return VCError::Success;
+  VCError e = ints_checked(src, n, name);
+  if (e == VCError::Success) e = ints_checked(dst, n, name);
+  for (int i = 0; i < n_layers && e == VCError::Success; ++i)
+    e = ready_to_launch(name, {layers[i].k, layers[i].v, layers[i].k_scale, layers[i].v_scale});
+  if (e == VCError::Success) e = ready_to_launch(name, {src, dst});
+  if (e != VCError::Success) return e;
+  return run(vcb::launch_kv8_copy(layers, n_layers, src, dst, n, s), name);
+}
+
+// A host structure (or array of them) passed as a Scalar argument.
+template <class T>
+bool arg_structs(const VCKernelArg *a, int n, int i, const T **out, int *count) {
+  if (i >= n || a[i].kind != VCKernelArg::Scalar || !a[i].data || !a[i].size ||
+      a[i].size % sizeof(T))
+    return false;
+  *out = static_cast<const T *>(a[i].data);
+  *count = (int)(a[i].size / sizeof(T));
+  return true;
+}
+bool arg_int(const VCKernelArg *a, int n, int i, int *out) {
+  long long v;
+  if (!arg_i64(a, n, i, &v) || v < INT32_MIN || v > INT32_MAX) return false;
+  *out = (int)v;
+  return true;
+}
+
+// vc.flash_window(Q, K, V, O, lens, strides, B, Hq, Hkv, Nq, Nk, d, window,
+// sinks, scale_log2, dtype): strides a Scalar of 12 int64 (Q, K, V, O).
+VCError k_native_flash_window(VCKernel &, const LaunchShape &, const VCKernelArg *a, int n,
+                              cudaStream_t s) {
+  vcb::FlashWindowArgs f{};
+  const void *o, *lens;
+  const int64_t *st12;
+  int count;
+  if (n != 16 || !arg_ptr(a, n, 0, &f.Q) || !arg_ptr(a, n, 1, &f.K) || !arg_ptr(a, n, 2, &f.V) ||
+      !arg_ptr(a, n, 3, &o) || !arg_ptr(a, n, 4, &lens) || !arg_structs(a, n, 5, &st12, &count) ||
+      count != 12 || !arg_int(a, n, 6, &f.B) || !arg_int(a, n, 7, &f.Hq) ||
+      !arg_int(a, n, 8, &f.Hkv) || !arg_int(a, n, 9, &f.Nq) || !arg_int(a, n, 10, &f.Nk) ||
+      !arg_int(a, n, 11, &f.d) || !arg_int(a, n, 12, &f.window) || !arg_int(a, n, 13, &f.sinks) ||
+      !arg_f32(a, n, 14, &f.scale_log2) || !arg_int(a, n, 15, &f.dtype))
+    return bad_args("vc.flash_window");
+  f.O = const_cast<void *>(o);
+  f.lens = static_cast<const int32_t *>(lens);
+  const int64_t *const strides[4] = {st12, st12 + 3, st12 + 6, st12 + 9};
+  return flash_window_checked(f, strides, s);
+}
+
+// vc.kv8_append(cache, K, V, k_stride, v_stride, tokens, table, table_width,
+// start, cu, B, max_new, lens_out, dtype): cache a Scalar vc_kv8_cache.
+VCError k_native_kv8_append(VCKernel &, const LaunchShape &, const VCKernelArg *a, int n,
+                            cudaStream_t s) {
+  vcb::Kv8AppendArgs g{};
+  int count;
+  long long ks, vs;
+  const void *table, *start, *cu, *lens;
+  if (n != 14 || !arg_structs(a, n, 0, &g.cache, &count) || count != 1 || !arg_ptr(a, n, 1, &g.K) ||
+      !arg_ptr(a, n, 2, &g.V) || !arg_i64(a, n, 3, &ks) || !arg_i64(a, n, 4, &vs) ||
+      !arg_int(a, n, 5, &g.T) || !arg_ptr(a, n, 6, &table) || !arg_int(a, n, 7, &g.table_width) ||
+      !arg_ptr(a, n, 8, &start) || !arg_ptr(a, n, 9, &cu) || !arg_int(a, n, 10, &g.B) ||
+      !arg_int(a, n, 11, &g.max_new) || !arg_ptr(a, n, 12, &lens) || !arg_int(a, n, 13, &g.dtype))
+    return bad_args("vc.kv8_append");
+  g.k_stride = ks;
+  g.v_stride = vs;
+  g.table = static_cast<const int32_t *>(table);
+  g.start = static_cast<const int32_t *>(start);
+  g.cu = static_cast<const int32_t *>(cu);
+  g.lens_out = static_cast<int32_t *>(const_cast<void *>(lens));
+  return kv8_append_checked(g, s);
+}
+
+// vc.kv8_attn(cache, Q, q_stride, O, o_stride, table, table_width, lens, B,
+// Hq, window, sinks, scale_log2, dtype, workspace, workspace_bytes)
+VCError k_native_kv8_attn(VCKernel &, const LaunchShape &, const VCKernelArg *a, int n,
+                          cudaStream_t s) {
+  vcb::Kv8AttnArgs g{};
+  int count;
+  long long qs, os, bytes;
+  const void *o, *table, *lens, *ws;
+  if (n != 16 || !arg_structs(a, n, 0, &g.cache, &count) || count != 1 || !arg_ptr(a, n, 1, &g.Q) ||
+      !arg_i64(a, n, 2, &qs) || !arg_ptr(a, n, 3, &o) || !arg_i64(a, n, 4, &os) ||
+      !arg_ptr(a, n, 5, &table) || !arg_int(a, n, 6, &g.table_width) || !arg_ptr(a, n, 7, &lens) ||
+      !arg_int(a, n, 8, &g.B) || !arg_int(a, n, 9, &g.Hq) || !arg_int(a, n, 10, &g.window) ||
+      !arg_int(a, n, 11, &g.sinks) || !arg_f32(a, n, 12, &g.scale_log2) ||
+      !arg_int(a, n, 13, &g.dtype) || !arg_ptr(a, n, 14, &ws) || !arg_i64(a, n, 15, &bytes) ||
+      bytes < 0)
+    return bad_args("vc.kv8_attn");
+  g.q_stride = qs;
+  g.o_stride = os;
+  g.O = const_cast<void *>(o);
+  g.table = static_cast<const int32_t *>(table);
+  g.lens = static_cast<const int32_t *>(lens);
+  g.workspace = const_cast<void *>(ws);
+  return kv8_attn_checked(g, (size_t)bytes, s);
+}
+
+// vc.kv8_copy_pages(layers, src, dst, n): layers a Scalar array of vc_kv8_cache.
+VCError k_native_kv8_copy(VCKernel &, const LaunchShape &, const VCKernelArg *a, int n,
+                          cudaStream_t s) {
+  const vc_kv8_cache *layers;
+  int n_layers, count;
+  const void *src, *dst;
+  if (n != 4 || !arg_structs(a, n, 0, &layers, &n_layers) || !arg_ptr(a, n, 1, &src) ||
+      !arg_ptr(a, n, 2, &dst) || !arg_int(a, n, 3, &count))
+    return bad_args("vc.kv8_copy_pages");
+  return kv8_copy_checked(layers, n_layers, static_cast<const int32_t *>(src),
+                          static_cast<const int32_t *>(dst), count, s);
+}
+
 const std::vector<KernelEntry> &registry() {
   static const std::vector<KernelEntry> r = {
       {"vadd", k_vadd, {}},
@@ -1473,6 +1752,10 @@ const std::vector<KernelEntry> &registry() {
       {"vc.block_reduce", k_native_block_reduce, {}},
       {"vc.gemm", k_native_gemm, {}},
       {"vc.flash_fwd", k_native_flash, {}},
+      {"vc.flash_window", k_native_flash_window, {}},
+      {"vc.kv8_append", k_native_kv8_append, {}},
+      {"vc.kv8_attn", k_native_kv8_attn, {}},
+      {"vc.kv8_copy_pages", k_native_kv8_copy, {}},
   };
   return r;
 }
@@ -1949,9 +2232,10 @@ int vc_kernel_set_constant(void *k, const char *name, long long value) {
 int vc_kernel_error(int clear) {
   if (!ensure_init()) return E(VCError::InitializationError);
   use_current_device();
-  int codes[5] = {vcb::stream_kernels_error(clear), vcb::gemm_tcgen05_error(clear),
+  int codes[8] = {vcb::stream_kernels_error(clear), vcb::gemm_tcgen05_error(clear),
                   vcb::gemm_f32_error(clear), vcb::flash_tcgen05_error(clear),
-                  vcb::selftest_error(clear)};
+                  vcb::selftest_error(clear), vcb::flash_window_error(clear),
+                  vcb::kv8_pages_error(clear), vcb::kv8_attn_error(clear)};
   for (int c : codes)
     if (c != 0) return c;
   return 0;
@@ -2127,6 +2411,55 @@ int vc_flash_fwd(const void *Q, const void *K, const void *V, void *O, int BH, i
   use_current_device();
   vcb::FlashArgs f{Q, K, V, O, BH, N, d, scale_log2, causal != 0, dtype};
   return E(flash_checked(f, reinterpret_cast<cudaStream_t>(s)));
+}
+
+int vc_flash_window_fwd(const void *Q, const void *K, const void *V, void *O, int B, int Hq,
+                        int Hkv, int Nq, int Nk, int d, const int64_t *q_strides,
+                        const int64_t *k_strides, const int64_t *v_strides,
+                        const int64_t *o_strides, const int32_t *lens, int window, int sinks,
+                        float scale_log2, int dtype, void *s) {
+  if (!Q || !K || !V || !O) return E(VCError::InvalidValue);
+  const cudaStream_t stream = resolve_stream(S(s));
+  ProfileScope prof("vc_flash_window_fwd", stream);
+  const vcb::FlashWindowArgs f{Q, K, V, O, B, Hq, Hkv, Nq, Nk, d, {}, {}, {}, {}, lens,
+                               window, sinks, scale_log2, dtype};
+  const int64_t *const strides[4] = {q_strides, k_strides, v_strides, o_strides};
+  return E(flash_window_checked(f, strides, stream));
+}
+int vc_kv8_append(const vc_kv8_cache *cache, const void *K, const void *V, int64_t k_stride,
+                  int64_t v_stride, int tokens, const int32_t *table, int table_width,
+                  const int32_t *start, const int32_t *cu, int B, int max_new,
+                  int32_t *lens_out, int dtype, void *s) {
+  if (!cache) return E(VCError::InvalidValue);
+  const cudaStream_t stream = resolve_stream(S(s));
+  ProfileScope prof("vc_kv8_append", stream);
+  return E(kv8_append_checked({cache, K, V, k_stride, v_stride, tokens, table, table_width, start,
+                               cu, B, max_new, lens_out, dtype}, stream));
+}
+int vc_kv8_attn_workspace(const vc_kv8_cache *cache, int B, int Hq, size_t *bytes) {
+  if (!cache || !bytes || B < 0 || Hq <= 0 || cache->heads <= 0 || Hq % cache->heads)
+    return E(VCError::InvalidValue);
+  if (!ensure_init()) return E(VCError::InitializationError);
+  use_current_device();
+  *bytes = vcb::kv8_attn_workspace_bytes(*cache, B, Hq);
+  return VC_SUCCESS;
+}
+int vc_kv8_attn(const vc_kv8_cache *cache, const void *Q, int64_t q_stride, void *O,
+                int64_t o_stride, const int32_t *table, int table_width, const int32_t *lens,
+                int B, int Hq, int window, int sinks, float scale_log2, int dtype,
+                void *workspace, size_t workspace_bytes, void *s) {
+  if (!cache) return E(VCError::InvalidValue);
+  const cudaStream_t stream = resolve_stream(S(s));
+  ProfileScope prof("vc_kv8_attn", stream);
+  return E(kv8_attn_checked({cache, Q, q_stride, O, o_stride, table, table_width, lens, B, Hq,
+                             window, sinks, scale_log2, dtype, workspace}, workspace_bytes, stream));
+}
+int vc_kv8_copy_pages(const vc_kv8_cache *layers, int n_layers, const int32_t *src,
+                      const int32_t *dst, int n, void *s) {
+  if (!layers) return E(VCError::InvalidValue);
+  const cudaStream_t stream = resolve_stream(S(s));
+  ProfileScope prof("vc_kv8_copy_pages", stream);
+  return E(kv8_copy_checked(layers, n_layers, src, dst, n, stream));
 }
 
 }  // extern "C"

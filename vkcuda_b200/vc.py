@@ -95,6 +95,7 @@ _lib: Optional[ctypes.CDLL] = None
 _VP, _SZ, _I, _U, _LL, _I64, _F = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint,
                                    ctypes.c_longlong, ctypes.c_int64, ctypes.c_float)
 _PVP, _PI = ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_int)
+_PI32, _PI64 = ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int64)
 HOSTFN = ctypes.CFUNCTYPE(None, ctypes.c_void_p)
 
 # name -> (restype, argtypes); every symbol of include/vc_b200.h.
@@ -153,6 +154,20 @@ SIGNATURES = {
     "vc_block_reduce_f32": (_I, [_VP, _VP, _I, _I, _I, _VP]),
     "vc_gemm": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I64, _I64, _I64, _I64, _I, _I, _VP]),
     "vc_flash_fwd": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _F, _I, _I, _VP]),
+    "vc_flash_window_fwd": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP, _VP, _VP,
+                                 _VP, _I, _I, _F, _I, _VP]),
+    "vc_kv8_append": (_I, [_VP, _VP, _VP, _I64, _I64, _I, _VP, _I, _VP, _VP, _I, _I, _VP, _I, _VP]),
+    "vc_kv8_attn_workspace": (_I, [_VP, _I, _I, ctypes.POINTER(_SZ)]),
+    "vc_kv8_attn": (_I, [_VP, _VP, _I64, _VP, _I64, _VP, _I, _VP, _I, _I, _I, _I, _F, _I, _VP, _SZ,
+                         _VP]),
+    "vc_kv8_copy_pages": (_I, [_VP, _I, _VP, _VP, _I, _VP]),
+    "vc_kv8_pool_create": (_I, [_PVP, _I, _I]), "vc_kv8_pool_destroy": (_I, [_VP]),
+    "vc_kv8_pool_new": (_I, [_VP, _PI64]), "vc_kv8_pool_fork": (_I, [_VP, _I64, _PI64]),
+    "vc_kv8_pool_extend": (_I, [_VP, _I64, _I64, _PI32, _PI32]),
+    "vc_kv8_pool_free": (_I, [_VP, _I64]),
+    "vc_kv8_pool_pages": (_I, [_VP, _I64, _VP, _I, _PI, _PI64]),
+    "vc_kv8_pool_info": (_I, [_VP, _PI, _PI]),
+    "vc_kv8_pool_compact": (_I, [_VP, _VP, _VP, _I, _PI]),
 }
 
 
@@ -566,3 +581,134 @@ def flash_fwd(Q, K, V, O, BH: int, N: int, d: int, scale_log2: float, causal: bo
     return VCError(library().vc_flash_fwd(_addr(Q), _addr(K), _addr(V), _addr(O), BH, N, d,
                                           float(scale_log2), 1 if causal else 0, int(dtype),
                                           _stream(stream)))
+
+
+# ------------------------------------------------------------ serving entries
+def _strides(s):
+    """Three element strides (batch, head, token), or None for a dense [B][H][N][d]."""
+    return None if s is None else (ctypes.c_int64 * 3)(*s)
+
+
+def flash_window_fwd(Q, K, V, O, B: int, Hq: int, Hkv: int, Nq: int, Nk: int, d: int,
+                     scale_log2: float, dtype: int, window: int = 0, sinks: int = 0, lens=None,
+                     q_strides=None, k_strides=None, v_strides=None, o_strides=None,
+                     stream=None) -> VCError:
+    """Causal attention of prompts through a sliding window with sinks, K/V heads
+    shared by groups of query heads (vc_flash_window_fwd)."""
+    return VCError(library().vc_flash_window_fwd(
+        _addr(Q), _addr(K), _addr(V), _addr(O), B, Hq, Hkv, Nq, Nk, d, _strides(q_strides),
+        _strides(k_strides), _strides(v_strides), _strides(o_strides), _addr(lens), window, sinks,
+        float(scale_log2), int(dtype), _stream(stream)))
+
+
+class Kv8Cache(ctypes.Structure):
+    """Byte-compatible with vc_kv8_cache (include/vc_b200.h): one layer of a paged
+    K/V cache in e4m3 codes with a scale per page and head."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("num_pages", ctypes.c_int), ("heads", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("page_stride", ctypes.c_int64), ("scale_stride", ctypes.c_int64)]
+
+
+def kv8_cache(k, v, k_scale, v_scale, num_pages: int, heads: int, page_size: int, head_dim: int,
+              page_stride: int = 0, scale_stride: int = 0) -> Kv8Cache:
+    """A layer's cache over device buffers that the caller keeps; strides 0: dense."""
+    return Kv8Cache(_addr(k), _addr(v), _addr(k_scale), _addr(v_scale), num_pages, heads, page_size,
+                    head_dim, page_stride or heads * page_size * head_dim, scale_stride or heads)
+
+
+def kv8_layers(caches: Sequence[Kv8Cache]):
+    """The layers of a model as vc_kv8_copy_pages takes them."""
+    return (Kv8Cache * len(caches))(*caches)
+
+
+def kv8_append(cache: Kv8Cache, K, V, tokens: int, table, table_width: int, start, B: int,
+               max_new: int, dtype: int, cu=None, lens_out=None, k_stride: int = 0,
+               v_stride: int = 0, stream=None) -> VCError:
+    """Quantise new K/V tokens into their sequences' pages (vc_kv8_append); strides 0: dense."""
+    row = cache.heads * cache.head_dim
+    return VCError(library().vc_kv8_append(
+        ctypes.byref(cache), _addr(K), _addr(V), k_stride or row, v_stride or row, tokens,
+        _addr(table), table_width, _addr(start), _addr(cu), B, max_new, _addr(lens_out), int(dtype),
+        _stream(stream)))
+
+
+def kv8_attn_workspace(cache: Kv8Cache, B: int, Hq: int) -> Tuple[VCError, int]:
+    """Bytes of workspace that kv8_attn needs for these sizes (zero it once)."""
+    n = ctypes.c_size_t(0)
+    e = library().vc_kv8_attn_workspace(ctypes.byref(cache), B, Hq, ctypes.byref(n))
+    return VCError(e), n.value
+
+
+def kv8_attn(cache: Kv8Cache, Q, O, table, table_width: int, lens, B: int, Hq: int,
+             scale_log2: float, dtype: int, workspace, workspace_bytes: int, window: int = 0,
+             sinks: int = 0, q_stride: int = 0, o_stride: int = 0, stream=None) -> VCError:
+    """Attention of one token for each sequence over the cache (vc_kv8_attn); strides 0: dense."""
+    row = Hq * cache.head_dim
+    return VCError(library().vc_kv8_attn(
+        ctypes.byref(cache), _addr(Q), q_stride or row, _addr(O), o_stride or row, _addr(table),
+        table_width, _addr(lens), B, Hq, window, sinks, float(scale_log2), int(dtype),
+        _addr(workspace), workspace_bytes, _stream(stream)))
+
+
+def kv8_copy_pages(layers, src, dst, n: int, stream=None) -> VCError:
+    """Copy pages src[i] -> dst[i] in every layer (kv8_layers), codes and scales."""
+    return VCError(library().vc_kv8_copy_pages(layers, len(layers), _addr(src), _addr(dst), n,
+                                               _stream(stream)))
+
+
+def kv8_pool_create(num_pages: int, page_size: int) -> Tuple[VCError, int]:
+    """Host bookkeeping of a cache's pages (vc_kv8_pool_create)."""
+    return _alloc(lambda p, _n: library().vc_kv8_pool_create(p, num_pages, page_size), 0)
+
+
+def kv8_pool_destroy(pool) -> VCError: return VCError(library().vc_kv8_pool_destroy(pool))
+
+
+def kv8_pool_new(pool) -> Tuple[VCError, int]:
+    s = ctypes.c_int64(0)
+    return VCError(library().vc_kv8_pool_new(pool, ctypes.byref(s))), s.value
+
+
+def kv8_pool_fork(pool, seq: int) -> Tuple[VCError, int]:
+    s = ctypes.c_int64(0)
+    return VCError(library().vc_kv8_pool_fork(pool, seq, ctypes.byref(s))), s.value
+
+
+def kv8_pool_extend(pool, seq: int, tokens: int) -> Tuple[VCError, Optional[Tuple[int, int]]]:
+    """Room for `tokens` more; (src, dst) is the page to copy first, None if there is none."""
+    a, b = ctypes.c_int32(-1), ctypes.c_int32(-1)
+    e = VCError(library().vc_kv8_pool_extend(pool, seq, tokens, ctypes.byref(a), ctypes.byref(b)))
+    return e, ((a.value, b.value) if e == VCError.Success and a.value >= 0 else None)
+
+
+def kv8_pool_free(pool, seq: int) -> VCError: return VCError(library().vc_kv8_pool_free(pool, seq))
+
+
+def kv8_pool_pages(pool, seq: int, pages=None, capacity: int = 0) -> Tuple[VCError, int, int]:
+    """A sequence's pages into `pages` (int32, -1 behind them up to `capacity`), and how many
+    pages and tokens it has."""
+    n, t = ctypes.c_int(0), ctypes.c_int64(0)
+    e = library().vc_kv8_pool_pages(pool, seq, _addr(pages), capacity, ctypes.byref(n),
+                                    ctypes.byref(t))
+    return VCError(e), n.value, t.value
+
+
+def kv8_pool_info(pool) -> Tuple[VCError, int, int]:
+    """Free pages and sequences."""
+    f, n = ctypes.c_int(0), ctypes.c_int(0)
+    return VCError(library().vc_kv8_pool_info(pool, ctypes.byref(f), ctypes.byref(n))), f.value, n.value
+
+
+def kv8_pool_compact(pool, copy_src, copy_dst, capacity: int) -> Tuple[VCError, int]:
+    """Move the held pages to the lowest numbers; the copies to make, in two int32 arrays."""
+    n = ctypes.c_int(0)
+    e = library().vc_kv8_pool_compact(pool, _addr(copy_src), _addr(copy_dst), capacity,
+                                      ctypes.byref(n))
+    return VCError(e), n.value
+
+
+def structs(v) -> Tuple[int, object]:
+    """A ctypes structure or array as a Scalar argument (the caches and strides of the serving
+    kernels)."""
+    return (VCKernelArg.SCALAR, v)
