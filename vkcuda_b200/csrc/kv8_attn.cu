@@ -50,8 +50,7 @@ namespace {
 constexpr int kTile = 64;      // keys per tile
 constexpr int kWarps = 4;      // 16 keys each
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 4;     // ring of a warp
-constexpr int kBlocksPerSm = 2;
+constexpr int kStages = 3;     // ring of a warp
 constexpr int kMaxHeads = 16;  // query heads of an item
 constexpr float kLazy = 8.0f;  // log2 units
 
@@ -63,7 +62,8 @@ struct Counters {
   unsigned group[2];  // of the group that starts with this block, by slot
   unsigned item;      // of the item that starts in this block
 };
-int grid_blocks() { return sm_count_current() * kBlocksPerSm; }
+constexpr int blocks_per_sm(int NT) { return NT == 1 ? 3 : 2; }
+int grid_blocks(int NT) { return sm_count_current() * blocks_per_sm(NT); }
 
 struct AttnParams {
   const uint8_t *k, *v;
@@ -170,7 +170,7 @@ struct Smem {
 };
 
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(const AttnParams p) {
   using S = Smem<D>;
   constexpr int NH = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -206,8 +206,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
     before = mine + s - x;
     return total;
   };
-  int seq_tiles = 0, before;
-  for (int b = tid; b < p.B; b += kThreads) seq_tiles += tiles_of(b);
+  const int mine = tid < p.B ? tiles_of(tid) : 0;
+  int seq_tiles = mine, before;
+  for (int b = tid + kThreads; b < p.B; b += kThreads) seq_tiles += tiles_of(b);
   const int all = block_scan(seq_tiles, before);
   const int64_t total = (int64_t)all * items;
   const int blocks = (int)(total < gridDim.x ? total : gridDim.x);
@@ -223,21 +224,23 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
   if ((int)blockIdx.x >= blocks) return;
   const int64_t t0 = split_start(total, blocks, blockIdx.x);
   const int64_t t1 = split_start(total, blocks, blockIdx.x + 1);
-  int64_t base = 0;  // tiles before the chunk of sequences, times items
   if (tid == 0) sh_found[0] = -1;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    const int n = b < p.B ? tiles_of(b) : 0;
-    const int chunk = block_scan(n, before);
-    if (t0 < base + (int64_t)chunk * items) {
-      const int64_t first = base + (int64_t)before * items;
-      if (t0 >= first && t0 < first + (int64_t)n * items) {
-        sh_found[0] = b;
-        sh_found[1] = (int)(t0 - first);
-      }
-      break;
+  __syncthreads();
+  auto found = [&](int b, int n, int64_t first) {
+    if (t0 < first || t0 >= first + (int64_t)n * items) return;
+    sh_found[0] = b;
+    sh_found[1] = (int)(t0 - first);
+  };
+  if (p.B <= kThreads) {
+    found(tid, mine, (int64_t)before * items);
+  } else {
+    int64_t base = 0;  // tiles before the chunk of sequences, times items
+    for (int b0 = 0; b0 < p.B && base <= t0; b0 += kThreads) {
+      const int n = b0 + tid < p.B ? tiles_of(b0 + tid) : 0;
+      const int chunk = block_scan(n, before);
+      found(b0 + tid, n, base + (int64_t)before * items);
+      base += (int64_t)chunk * items;
     }
-    base += (int64_t)chunk * items;
   }
   __syncthreads();
   if (sh_found[0] < 0) return;
@@ -254,12 +257,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
   auto any_visible = [&](const Cursor &c, int k0) {
     return k0 < c.vis.len && (k0 + 15 >= c.vis.lo || k0 < c.vis.sink);
   };
-  // The page of the next copy is looked up one step ahead of it.
-  int page = -1;
+  // Pages of 32 tiles of the item from `pages_at` on, one per lane.
+  int pages = -1, pages_at = 0;
   auto look_up = [&]() {
-    if (pre_t >= t1) return;
-    const int k0 = first_key(pre);
-    if (any_visible(pre, k0)) page = __ldg(p.table + (int64_t)pre.b * p.table_width + (k0 >> p.page_shift));
+    pages_at = pre.tile;
+    const int i = pre.tile + lane;
+    if (i >= pre.tiles.count) return;
+    const int k0 = tile_key(pre.tiles, i, kTile) + warp * 16;
+    if (any_visible(pre, k0)) pages = __ldg(p.table + (int64_t)pre.b * p.table_width + (k0 >> p.page_shift));
   };
   auto issue = [&](int stage) {
     if (pre_t < t1) {
@@ -267,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
       const int k0 = first_key(pre);
       uint32_t mask = 0;
       if (any_visible(pre, k0)) {
+        const int page = __shfl_sync(0xffffffffu, pages, pre.tile - pages_at);
         const bool bad = page < 0 || page >= p.num_pages;
         if (bad && lane == 0) record_error(kErrOutOfBounds);
         mask = __ballot_sync(0xffffffffu, !bad && lane < 16 && key_visible(pre.vis, k0 + lane));
@@ -292,8 +298,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
       }
       if (lane == 0) *reinterpret_cast<uint32_t *>(at + 32 * D + 8) = mask;
       ++pre_t;
-      if (++pre.tile == pre.tiles.count && pre_t < t1) next_item(pre, p);
-      look_up();
+      const bool turn = ++pre.tile == pre.tiles.count;
+      if (turn && pre_t < t1) next_item(pre, p);
+      if (turn || pre.tile - pages_at == 32) look_up();
     }
     cp_async_commit();
   };
@@ -374,9 +381,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
       if (mask == 0) continue;  // uniform over the warp
       const float ks = __uint_as_float(meta.x), vs = __uint_as_float(meta.y);
 
-      float s[NT][4];
+      float s[NT][4], s2[NT][4];  // even and odd steps of d: two shorter chains of products
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[nt][x] = s2[nt][x] = 0.0f;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         const int sw = D == 128 ? (r & 1) << 2 : 0;  // rows r and r + 8 alike
@@ -389,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
                          a3 = half2_hi(wh[j]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma16816(s[nt], a0, a1, a2, a3, q[nt][4 * c + j][0], q[nt][4 * c + j][1]);
+            mma16816(j & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, q[nt][4 * c + j][0], q[nt][4 * c + j][1]);
         }
       }
       // Scores in log2 units; hidden keys -inf.
@@ -403,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          s[nt][x] = on0 ? s[nt][x] * (mult[nt][x] * ks) : -INFINITY;
-          s[nt][2 + x] = on1 ? s[nt][2 + x] * (mult[nt][x] * ks) : -INFINITY;
+          s[nt][x] = on0 ? (s[nt][x] + s2[nt][x]) * (mult[nt][x] * ks) : -INFINITY;
+          s[nt][2 + x] = on1 ? (s[nt][2 + x] + s2[nt][2 + x]) * (mult[nt][x] * ks) : -INFINITY;
           grow |= fmaxf(s[nt][x], s[nt][2 + x]) + lv > m[nt][x] + kLazy;
         }
       if (__any_sync(0xffffffffu, grow)) {
@@ -548,50 +557,62 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
       if (parts > 8)
         for (size = 3; size * size < parts;) ++size;
       const int groups = (parts + size - 1) / size;
-      auto slot_of = [&](int part) {  // part's slot: its range starts within the item, or the item in it
-        const int c = first + part;
-        return (size_t)c * 2 + (split_start(total, blocks, c) >= item0 ? 0 : 1);
-      };
-      // Joins parts a, a + step, ... below b into `out`, or into part a's slot.
-      auto join = [&](int a, int b, int step, bool to_out) {
+      // A part's slot: 1 where the item starts within the block's range.
+      const int first_slot = split_start(total, blocks, first) < item0 ? 1 : 0;
+      auto slot_of = [&](int part) { return (size_t)(first + part) * 2 + (part ? 0 : first_slot); };
+      // Joins the n parts a, a + step, ... into the output, or into part a's slot.
+      auto join = [&](int a, int n, int step, bool to_out) {
         __threadfence();
-        for (int e = tid; e < NH * D / 4; e += kThreads) {
-          const int h = e / (D / 4), d = e % (D / 4) * 4;
+        float *w = merge_o;  // [n][NH] weights, then [NH] sums
+        for (int e = tid; e < n * NH; e += kThreads) {
+          const float *from = p.slots + slot_of(a + e / NH * step) * kSlotFloats + NH * D;
+          w[e] = __ldcg(from + 2 * (e % NH));
+          w[(n + 1) * NH + e] = __ldcg(from + 2 * (e % NH) + 1);
+        }
+        __syncthreads();
+        if (tid < NH) {
           float mm = -INFINITY, sum = 0.0f;
-          float4 acc = make_float4(0, 0, 0, 0);
-          for (int q2 = a; q2 < b; q2 += step) {
-            const float *from = p.slots + slot_of(q2) * kSlotFloats;
-            const float mw = __ldcg(from + NH * D + 2 * h), lw = __ldcg(from + NH * D + 2 * h + 1);
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + h * D + d));
-            const float mn = fmaxf(mm, mw);
-            const float fo = mm == -INFINITY ? 1.0f : ex2_approx(mm - mn);
-            const float f = mw == -INFINITY ? 1.0f : ex2_approx(mw - mn);
-            acc = make_float4(acc.x * fo + f * x.x, acc.y * fo + f * x.y, acc.z * fo + f * x.z,
-                              acc.w * fo + f * x.w);
-            sum = sum * fo + f * lw;
-            mm = mn;
+          for (int i = 0; i < n; ++i) mm = fmaxf(mm, w[i * NH + tid]);
+          for (int i = 0; i < n; ++i) {
+            const float mi = w[i * NH + tid];
+            // Of a part without a visible key: 0 and 0, or NaN.
+            const float f = mi == -INFINITY ? 1.0f : ex2_approx(mi - mm);
+            w[i * NH + tid] = f;
+            sum += f * w[(n + 1 + i) * NH + tid];
           }
-          if (to_out) {
-            write_out(h, d, acc, sum);
-          } else {
-            merge_o[h * D + d] = acc.x;  // the slots are read by other threads still
-            merge_o[h * D + d + 1] = acc.y;
-            merge_o[h * D + d + 2] = acc.z;
-            merge_o[h * D + d + 3] = acc.w;
-            if (d == 0) {
-              merge_m[h] = mm;
-              merge_l[h] = sum;
-            }
+          w[n * NH + tid] = sum;
+          merge_m[tid] = mm;
+        }
+        __syncthreads();
+        constexpr int kVecs = NH * D / 4 / kThreads;
+        float4 acc[kVecs];
+#pragma unroll
+        for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+          const float *from = p.slots + slot_of(a + i * step) * kSlotFloats;
+#pragma unroll
+          for (int x = 0; x < kVecs; ++x) {
+            const int e = tid + x * kThreads;
+            const float f = w[i * NH + e / (D / 4)];
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(from) + e);
+            acc[x] = make_float4(acc[x].x + f * v.x, acc[x].y + f * v.y, acc[x].z + f * v.z,
+                                 acc[x].w + f * v.w);
           }
         }
-        if (!to_out) {
-          __syncthreads();
-          float *to = p.slots + slot_of(a) * kSlotFloats;
-          for (int e = tid; e < NH * D; e += kThreads) __stcg(to + e, merge_o[e]);
-          for (int h = tid; h < NH; h += kThreads) {
-            __stcg(to + NH * D + 2 * h, merge_m[h]);
-            __stcg(to + NH * D + 2 * h + 1, merge_l[h]);
-          }
+        if (!to_out) __syncthreads();  // every thread has read part a's slot
+        float *to = p.slots + slot_of(a) * kSlotFloats;
+#pragma unroll
+        for (int x = 0; x < kVecs; ++x) {
+          const int e = tid + x * kThreads, h = e / (D / 4);
+          if (to_out)
+            write_out(h, e % (D / 4) * 4, acc[x], w[n * NH + h]);
+          else
+            __stcg(reinterpret_cast<float4 *>(to) + e, acc[x]);
+        }
+        if (!to_out && tid < NH) {
+          __stcg(to + NH * D + 2 * tid, merge_m[tid]);
+          __stcg(to + NH * D + 2 * tid + 1, w[n * NH + tid]);
         }
       };
       // Counts this block in; true for the one that completes `of`.
@@ -610,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv8_attn_kernel(const 
       const int ga = g * size, gb = min(ga + size, parts);
       const size_t lead = slot_of(ga);
       if (arrive(&p.counters[lead >> 1].group[lead & 1], gb - ga)) {
-        join(ga, gb, 1, groups == 1);
-        if (groups > 1 && arrive(&p.counters[first].item, groups)) join(0, parts, size, true);
+        join(ga, gb - ga, 1, groups == 1);
+        if (groups > 1 && arrive(&p.counters[first].item, groups)) join(0, groups, size, true);
       }
     }
     __syncthreads();  // the merge buffer is free again
@@ -638,14 +659,14 @@ cudaError_t launch_typed(const AttnParams &p, cudaStream_t stream) {
       if (dev < 64) configured |= (1ull << dev);
     }
   }
-  kv8_attn_kernel<D, NT, BF16><<<grid_blocks(), kThreads, bytes, stream>>>(p);
+  kv8_attn_kernel<D, NT, BF16><<<grid_blocks(NT), kThreads, bytes, stream>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 size_t kv8_attn_workspace_bytes(const vc_kv8_cache &, int, int) {
-  const size_t blocks = grid_blocks();
+  const size_t blocks = grid_blocks(1);
   return blocks * (2 * kSlotFloats * sizeof(float) + sizeof(Counters));
 }
 
@@ -663,7 +684,7 @@ cudaError_t launch_kv8_attn(const Kv8AttnArgs &a, cudaStream_t stream) {
   const AttnParams p{static_cast<const uint8_t *>(c.k), static_cast<const uint8_t *>(c.v),
                      c.k_scale, c.v_scale, c.page_stride, c.scale_stride, a.q_stride, a.o_stride,
                      a.Q, a.O, a.table, a.lens, slots,
-                     reinterpret_cast<Counters *>(slots + grid_blocks() * 2 * kSlotFloats),
+                     reinterpret_cast<Counters *>(slots + (size_t)grid_blocks(1) * 2 * kSlotFloats),
                      a.B, c.num_pages, shift, c.heads, group, groups, a.table_width, a.window,
                      a.sinks, a.scale_log2};
   const bool bf16 = a.dtype == VC_DTYPE_BF16;
