@@ -9,7 +9,7 @@
 // query heads that share a K/V head are the columns of one matrix product.
 //
 // Split. The visible keys of every (sequence, K/V head, group of up to 8 NT
-// query heads) - an item - are cut into tiles of 64 keys, and all tiles of the
+// query heads) - an item - are cut into tiles of 128 keys, and all tiles of the
 // batch, in order, into equal contiguous ranges, one per block of a grid that
 // fills the GPU once: ragged batches load every SM alike whatever the lengths
 // are, which only the device knows. An item that lies within one block is
@@ -18,14 +18,15 @@
 // result does not depend on which that is), over groups of blocks first when
 // they are many.
 //
-// A warp takes 16 of a tile's 64 keys, through a ring of its own: 16-byte
-// asynchronous copies of the keys' codes (rows that the mask hides are
-// zero-filled and not read, so what they hold does not matter) and of the
-// page's two scales; warps of a block meet only where an item ends. Per 16
-// keys, with m16n8k16 fp16 products and fp32 accumulators:
+// A warp takes 32 of a tile's 128 keys, through a ring of its own that TMA
+// fills: boxes of 16 or 32 rows of the page's codes, swizzled so that the
+// reads below meet no bank twice. Warps of a block meet only where an item
+// ends. Rows that the mask hides arrive too; their scores become minus
+// infinity and their values zero, whatever they hold. Per 16 keys, with
+// m16n8k16 fp16 products and fp32 accumulators:
 //   S^T = K Q^T   A = the codes as fp16 (exact), rows keys; B = q. The order of
 //                 d within the product is free, so that a thread's operands are
-//                 16 contiguous bytes of a row.
+//                 16 contiguous bytes of a row; so is the order of the keys.
 //   P^T           8 x 8 transposes (movmatrix) of the fp16 weights.
 //   O^T += V^T P^T   A = pairs of keys' codes interleaved by byte permutes.
 // bf16 queries are scaled by a power of two per row into fp16's range (exact
@@ -47,10 +48,9 @@
 namespace vcb {
 namespace {
 
-constexpr int kTile = 64;      // keys per tile
-constexpr int kWarps = 4;      // 16 keys each
+constexpr int kTile = 128;     // keys per tile
+constexpr int kWarps = 4;      // 32 keys each
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;     // ring of a warp
 constexpr int kMaxHeads = 16;  // query heads of an item
 constexpr float kLazy = 8.0f;  // log2 units
 
@@ -66,9 +66,9 @@ constexpr int blocks_per_sm(int NT) { return NT == 1 ? 3 : 2; }
 int grid_blocks(int NT) { return sm_count_current() * blocks_per_sm(NT); }
 
 struct AttnParams {
-  const uint8_t *k, *v;
+  CUtensorMap k, v;  // (d, heads * page_size, pages)
   const float *k_scale, *v_scale;
-  int64_t page_stride, scale_stride, q_stride, o_stride;
+  int64_t scale_stride, q_stride, o_stride;
   const void *Q;
   void *O;
   const int32_t *table, *lens;
@@ -78,21 +78,6 @@ struct AttnParams {
   float scale_log2;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -158,29 +143,47 @@ __device__ __forceinline__ void next_item(Cursor &c, const AttnParams &p) {
   while (c.tiles.count == 0 && c.b + 1 < p.B) set_sequence(c, p, c.b + 1);
 }
 
-template <int D>
+template <int D, int NT>
 struct Smem {
-  static constexpr int kStageBytes = 2 * 16 * D + 16;  // K rows, V rows, scales, mask
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kRow = D + 4;  // floats of a head's row in the merge
-  template <int NT>
-  static constexpr int bytes() {
-    return kRing + kWarps * 8 * NT * (kRow + 2) * 4;
-  }
+  static constexpr int kHalf = 16 * D;       // 16 keys' codes of K or V
+  static constexpr int kStage = 4 * kHalf;   // K, K, V, V
+  static constexpr int kStages = 16384 / kStage;  // ring of a warp
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kMetas = kRing;       // of every stage
+  static constexpr int kBars = kMetas + kWarps * kStages * 32;
+  static constexpr int kMerge = kBars + ((kWarps * kStages * 8 + 15) & ~15);
+  static constexpr int kMergeWarp = 32 * (D * NT / 4 + 4 * NT);  // floats a warp hands over
+  static constexpr int kBytes = kMerge + 2 * kMergeWarp * 4 + 1024;  // the ring 1024-byte aligned
 };
+struct alignas(16) Meta {
+  float k_scale[2], v_scale[2];  // of the halves
+  uint32_t mask;                 // visible keys
+};
+static_assert(sizeof(Meta) == 32, "two 16-byte words a stage");
+
+// The low n bits.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+}
 
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(const AttnParams p) {
-  using S = Smem<D>;
-  constexpr int NH = 8 * NT;
-  extern __shared__ __align__(128) uint8_t smem[];
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT))
+kv8_attn_kernel(const __grid_constant__ AttnParams p) {
+  using S = Smem<D, NT>;
+  constexpr int NH = 8 * NT, kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *const smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int sh_scan[kWarps], sh_found[2];
   __shared__ unsigned sh_last;
-  float *merge_o = reinterpret_cast<float *>(smem + S::kRing);    // [warp][NH][kRow]
-  float *merge_m = merge_o + kWarps * NH * S::kRow;               // [warp][NH]
-  float *merge_l = merge_m + kWarps * NH;
+  float *const merge = reinterpret_cast<float *>(smem + S::kMerge);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, t = lane & 3;
+  uint64_t *const full = reinterpret_cast<uint64_t *>(smem + S::kBars) + warp * kStages;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
   const int items = p.heads * p.groups;
 
   // ---- this block's range of tiles
@@ -250,63 +253,87 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(c
   cur.tile = sh_found[1] % cur.tiles.count;
 
   // ---- the warp's ring
-  uint8_t *ring = smem + warp * kStages * S::kStageBytes;
+  uint8_t *const ring = smem + warp * kStages * S::kStage;
+  Meta *const metas = reinterpret_cast<Meta *>(smem + S::kMetas + warp * kStages * 32);
+  const bool two = p.page_shift == 4;  // pages of 16 tokens: two per step
   Cursor pre = cur;
   int64_t pre_t = t0;
-  auto first_key = [&](const Cursor &c) { return tile_key(c.tiles, c.tile, kTile) + warp * 16; };
-  auto any_visible = [&](const Cursor &c, int k0) {
-    return k0 < c.vis.len && (k0 + 15 >= c.vis.lo || k0 < c.vis.sink);
+  auto any_visible = [&](const Cursor &c, int k0, int n) {
+    return k0 < c.vis.len && (k0 + n - 1 >= c.vis.lo || k0 < c.vis.sink);
   };
-  // Pages of 32 tiles of the item from `pages_at` on, one per lane.
-  int pages = -1, pages_at = 0;
+  // Pages of the item's tiles from `pages_at` on, one tile per lane, and their
+  // scales; a lane issues the copies of its own tile.
+  int pages[2] = {-1, -1}, pages_at = 0;
+  float scales[4];
   auto look_up = [&]() {
     pages_at = pre.tile;
     const int i = pre.tile + lane;
-    if (i >= pre.tiles.count) return;
-    const int k0 = tile_key(pre.tiles, i, kTile) + warp * 16;
-    if (any_visible(pre, k0)) pages = __ldg(p.table + (int64_t)pre.b * p.table_width + (k0 >> p.page_shift));
+    pages[0] = pages[1] = -1;
+    scales[0] = scales[1] = scales[2] = scales[3] = 0.0f;
+    if (i >= pre.tiles.count || pre_t >= t1) return;
+    const int k0 = tile_key(pre.tiles, i, kTile) + warp * 32;
+    const int32_t *row = p.table + (int64_t)pre.b * p.table_width;
+    const int head = pre.item / p.groups;
+    bool bad = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!any_visible(pre, k0 + 16 * h, 16)) continue;
+      pages[h] = __ldg(row + ((k0 + 16 * h) >> p.page_shift));
+      if (pages[h] < 0 || pages[h] >= p.num_pages) {
+        pages[h] = -1;
+        bad = true;
+      } else {
+        scales[h] = __ldg(p.k_scale + pages[h] * p.scale_stride + head);
+        scales[2 + h] = __ldg(p.v_scale + pages[h] * p.scale_stride + head);
+      }
+    }
+    if (bad) record_error(kErrOutOfBounds);
   };
   auto issue = [&](int stage) {
-    if (pre_t < t1) {
-      uint8_t *at = ring + stage * S::kStageBytes;
-      const int k0 = first_key(pre);
-      uint32_t mask = 0;
-      if (any_visible(pre, k0)) {
-        const int page = __shfl_sync(0xffffffffu, pages, pre.tile - pages_at);
-        const bool bad = page < 0 || page >= p.num_pages;
-        if (bad && lane == 0) record_error(kErrOutOfBounds);
-        mask = __ballot_sync(0xffffffffu, !bad && lane < 16 && key_visible(pre.vis, k0 + lane));
-        if (!bad) {
-          const int head = pre.item / p.groups;
-          const int64_t off = page * p.page_stride +
-                              (((int64_t)head << p.page_shift) + (k0 & ((1 << p.page_shift) - 1))) * D;
-          constexpr int kChunks = D / 16;  // of a row
+    if (pre_t >= t1) return;
+    if (lane == pre.tile - pages_at) {
+      const int k0 = tile_key(pre.tiles, pre.tile, kTile) + warp * 32;
+      uint32_t mask = low_bits(pre.vis.len - k0) &
+                      (~low_bits(pre.vis.lo - k0) | low_bits(pre.vis.sink - k0));
+      if (pages[0] < 0) mask &= 0xffff0000u;
+      if (pages[1] < 0) mask &= 0x0000ffffu;
+      Meta &m = metas[stage];
+      m.k_scale[0] = scales[0];
+      m.k_scale[1] = scales[1];
+      m.v_scale[0] = scales[2];
+      m.v_scale[1] = scales[3];
+      m.mask = mask;
+      uint8_t *at = ring + stage * S::kStage;
+      const int row = ((pre.item / p.groups) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
+      if (two) {
+        const int n = (pages[0] >= 0) + (pages[1] >= 0);
+        mbar_arrive_expect_tx(&full[stage], n * 2 * S::kHalf);
 #pragma unroll
-          for (int i = 0; i < kChunks / 2; ++i) {
-            const int row = (i * 32 + lane) / kChunks, ch = lane % kChunks;
-            const uint32_t bytes = mask >> row & 1 ? 16 : 0;
-            const int64_t src = off + row * D + ch * 16;
-            const int swk = D == 128 ? (row & 1) << 2 : 0;
-            const int swv = D == 128 ? ((row >> 1) & 3) << 1 : (row >> 1) & 3;
-            cp_async16(smem_u32(at + row * D + (ch ^ swk) * 16), p.k + src, bytes);
-            cp_async16(smem_u32(at + 16 * D + row * D + (ch ^ swv) * 16), p.v + src, bytes);
+        for (int h = 0; h < 2; ++h)
+          if (pages[h] >= 0) {
+            tma_load_3d(at + h * S::kHalf, &p.k, 0, row, pages[h], &full[stage]);
+            tma_load_3d(at + (2 + h) * S::kHalf, &p.v, 0, row, pages[h], &full[stage]);
           }
-          if (lane < 2)
-            cp_async4(smem_u32(at + 32 * D + lane * 4),
-                      (lane ? p.v_scale : p.k_scale) + page * p.scale_stride + head, 4);
+      } else {
+        const int page = max(pages[0], pages[1]);
+        mbar_arrive_expect_tx(&full[stage], page >= 0 ? S::kStage : 0);
+        if (page >= 0) {
+          tma_load_3d(at, &p.k, 0, row, page, &full[stage]);
+          tma_load_3d(at + 2 * S::kHalf, &p.v, 0, row, page, &full[stage]);
         }
       }
-      if (lane == 0) *reinterpret_cast<uint32_t *>(at + 32 * D + 8) = mask;
-      ++pre_t;
-      const bool turn = ++pre.tile == pre.tiles.count;
-      if (turn && pre_t < t1) next_item(pre, p);
-      if (turn || pre.tile - pages_at == 32) look_up();
     }
-    cp_async_commit();
+    ++pre_t;
+    const bool turn = ++pre.tile == pre.tiles.count;
+    if (turn && pre_t < t1) next_item(pre, p);
+    if (turn || pre.tile - pages_at == 32) look_up();
   };
+  __syncwarp();
   look_up();
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < kStages - 1; ++s) issue(s);
+  uint32_t phase = 0;
+  bool ok = true;
 
   int stage = 0;
   for (int64_t at_tile = t0; at_tile < t1;) {
@@ -371,57 +398,91 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(c
     const int n = (int)(left < cur.tiles.count - cur.tile ? left : cur.tiles.count - cur.tile);
     if (n <= 0) break;
     for (int i = 0; i < n; ++i) {
-      cp_async_wait<kStages - 2>();
+      if (!ok) break;
       __syncwarp();
       issue(stage == 0 ? kStages - 1 : stage - 1);
-      const uint32_t at = smem_u32(ring + stage * S::kStageBytes);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-      const uint4 meta = lds128(at + 32 * D);
-      const uint32_t mask = meta.z;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase));
+      if (!ok) break;
+      const uint32_t at = smem_u32(ring + stage * S::kStage);
+      const uint4 sc = lds128(smem_u32(&metas[stage]));
+      const uint32_t mask = metas[stage].mask;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
       if (mask == 0) continue;  // uniform over the warp
-      const float ks = __uint_as_float(meta.x), vs = __uint_as_float(meta.y);
+      const float ks[2] = {__uint_as_float(sc.x), __uint_as_float(sc.y)};
+      const float vs[2] = {__uint_as_float(sc.z), __uint_as_float(sc.w)};
 
-      float s[NT][4], s2[NT][4];  // even and odd steps of d: two shorter chains of products
+      // Row x of the product is key x of the half in an order in which the 8
+      // lanes that a shared-memory read serves at once meet different banks:
+      // even rows 2i take key 2i, odd rows 2i + 1 key (2i ^ 4) + 1.
+      const int key_r = r & 1 ? ((r - 1) ^ 4) + 1 : r;
+      float s[2][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[nt][x] = s2[nt][x] = 0.0f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[h][nt][x] = 0.0f;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        const int sw = D == 128 ? (r & 1) << 2 : 0;  // rows r and r + 8 alike
-        const uint4 lo = lds128(at + r * D + ((4 * c + t) ^ sw) * 16);
-        const uint4 hi = lds128(at + (r + 8) * D + ((4 * c + t) ^ sw) * 16);
-        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+        const int ch = (4 * c + t) ^ (D == 128 ? key_r & 7 : (key_r >> 1) & 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t a0 = half2_lo(wl[j]), a1 = half2_lo(wh[j]), a2 = half2_hi(wl[j]),
-                         a3 = half2_hi(wh[j]);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t from = at + h * S::kHalf + key_r * D + ch * 16;
+          const uint4 lo = lds128(from), hi = lds128(from + 8 * D);
+          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(j & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, q[nt][4 * c + j][0], q[nt][4 * c + j][1]);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a0 = half2_lo(wl[j]), a1 = half2_lo(wh[j]), a2 = half2_hi(wl[j]),
+                           a3 = half2_hi(wh[j]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(s[h][nt], a0, a1, a2, a3, q[nt][4 * c + j][0], q[nt][4 * c + j][1]);
+          }
         }
       }
       // Scores in log2 units; hidden keys -inf.
-      const bool on0 = mask >> r & 1, on1 = mask >> (r + 8) & 1;
-      // log2 of the value scale: for the maximum kept from minus infinity, for
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[h][nt][x] *= mult[nt][x & 1] * ks[h];
+      if (mask != 0xffffffffu) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (!(mask >> (16 * h + key_r + (x >> 1) * 8) & 1)) s[h][nt][x] = -INFINITY;
+      }
+      // log2 of the value scales: for the maximum kept from minus infinity, for
       // the weights not (a zero scale takes its values out).
-      const float lv = vs > 0.0f ? fmaxf(lg2_approx(vs), -110.0f) : -110.0f;
-      const float lvp = vs > 0.0f ? lv : -INFINITY;
+      float lv[2], lvp[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        lv[h] = vs[h] > 0.0f ? fmaxf(lg2_approx(vs[h]), -110.0f) : -110.0f;
+        lvp[h] = vs[h] > 0.0f ? lv[h] : -INFINITY;
+      }
+      float top[NT][2];
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          s[nt][x] = on0 ? (s[nt][x] + s2[nt][x]) * (mult[nt][x] * ks) : -INFINITY;
-          s[nt][2 + x] = on1 ? (s[nt][2 + x] + s2[nt][2 + x]) * (mult[nt][x] * ks) : -INFINITY;
-          grow |= fmaxf(s[nt][x], s[nt][2 + x]) + lv > m[nt][x] + kLazy;
+          top[nt][x] = fmaxf(fmaxf(s[0][nt][x], s[0][nt][2 + x]) + lv[0],
+                             fmaxf(s[1][nt][x], s[1][nt][2 + x]) + lv[1]);
+          grow |= top[nt][x] > m[nt][x] + kLazy;
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float mx = fmaxf(s[nt][x], s[nt][2 + x]) + lv;
+            float mx = top[nt][x];
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -436,115 +497,150 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(c
             }
           }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
+        const float mm[2] = {m[nt][0] == -INFINITY ? 0.0f : m[nt][0],
+                             m[nt][1] == -INFINITY ? 0.0f : m[nt][1]};
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float mm = m[nt][x] == -INFINITY ? 0.0f : m[nt][x];
-          w[x] = ex2_approx(s[nt][x] + (lvp - mm));
-          w[2 + x] = ex2_approx(s[nt][2 + x] + (lvp - mm));
-          l[nt][x] += ex2_approx(s[nt][x] - mm) + ex2_approx(s[nt][2 + x] - mm);
-        }
-        pb[nt][0] = transpose8x8(pack_half2(w[0], w[1]));
-        pb[nt][1] = transpose8x8(pack_half2(w[2], w[3]));
-      }
-      // Values: this thread's keys 2t, 2t + 1, 2t + 8, 2t + 9, D / 8 codes from d = r D / 8 on.
-      uint32_t v[4][D / 32];
+        for (int h = 0; h < 2; ++h) {
+          float w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-        if constexpr (D == 128) {
-          const uint4 w = lds128(at + 16 * D + key * D + ((r ^ (t << 1)) * 16));
-          v[k][0] = w.x;
-          v[k][1] = w.y;
-          v[k][2] = w.z;
-          v[k][3] = w.w;
-        } else {
-          const uint2 w = lds64(at + 16 * D + key * D + ((r >> 1) ^ t) * 16 + (r & 1) * 8);
-          v[k][0] = w.x;
-          v[k][1] = w.y;
+          for (int x = 0; x < 4; ++x) {
+            w[x] = ex2_approx(s[h][nt][x] + (lvp[h] - mm[x & 1]));
+            l[nt][x & 1] += ex2_approx(s[h][nt][x] - mm[x & 1]);
+          }
+          pb[h][nt][0] = transpose8x8(pack_half2(w[0], w[1]));
+          pb[h][nt][1] = transpose8x8(pack_half2(w[2], w[3]));
         }
       }
+      // Values: rows 2t, 2t + 1, 2t + 8, 2t + 9, D / 8 codes from d = r D / 8 on.
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j)
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[4][D / 32];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362 : 0x5140;
-          const uint32_t ab = __byte_perm(v[0][j], v[1][j], sel), cd = __byte_perm(v[2][j], v[3][j], sel);
-          const uint32_t a0 = half2_lo(ab), a1 = half2_hi(ab), a2 = half2_lo(cd), a3 = half2_hi(cd);
+        for (int k = 0; k < 4; ++k) {
+          const int key = (k & 1 ? ((2 * t) ^ 4) + 1 : 2 * t) + (k >> 1) * 8;
+          const uint32_t row = at + (2 + h) * S::kHalf + key * D;
+          if constexpr (D == 128) {
+            const uint4 w = lds128(row + ((r ^ (key & 7)) * 16));
+            v[k][0] = w.x;
+            v[k][1] = w.y;
+            v[k][2] = w.z;
+            v[k][3] = w.w;
+          } else {
+            const uint2 w = lds64(row + (((r >> 1) ^ ((key >> 1) & 3)) * 16) + (r & 1) * 8);
+            v[k][0] = w.x;
+            v[k][1] = w.y;
+          }
+          if (mask != 0xffffffffu && !(mask >> (16 * h + key) & 1)) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(o[nt][2 * j + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            for (int j = 0; j < D / 32; ++j) v[k][j] = 0;
+          }
         }
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t sel = u ? 0x7362 : 0x5140;
+            const uint32_t ab = __byte_perm(v[0][j], v[1][j], sel), cd = __byte_perm(v[2][j], v[3][j], sel);
+            const uint32_t a0 = half2_lo(ab), a1 = half2_hi(ab), a2 = half2_lo(cd), a3 = half2_hi(cd);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(o[nt][2 * j + u], a0, a1, a2, a3, pb[h][nt][0], pb[h][nt][1]);
+          }
+      }
     }
 
-    // ---- the warps' results joined
+    // ---- the warps' results joined: 2 and 3 into 0 and 1, then 1 into 0, each
+    // thread's registers through shared memory to the same lane of the other.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float sum = l[nt][x];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        const int col = nt * 8 + 2 * t + x;
-        if (r == 0) {
-          merge_m[warp * NH + col] = m[nt][x];
-          merge_l[warp * NH + col] = sum;
-        }
-        // d = r D / 8 + 2 i, + 1 of fragment i.
-        float *to = merge_o + (warp * NH + col) * S::kRow + r * (D / 8);
-#pragma unroll
-        for (int i = 0; i < D / 16; i += 2)
-          *reinterpret_cast<float4 *>(to + 2 * i) =
-              make_float4(o[nt][i][x], o[nt][i][2 + x], o[nt][i + 1][x], o[nt][i + 1][2 + x]);
+        l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 4);
+        l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 8);
+        l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 16);
       }
-    __syncthreads();
+    constexpr int kFrags = D / 16 * NT;  // float4 of O per thread
+#pragma unroll
+    for (int half = kWarps / 2; half; half >>= 1) {
+      float4 *const buf = reinterpret_cast<float4 *>(merge + (warp % half) * S::kMergeWarp) + lane;
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            buf[(nt * (D / 16) + i) * 32] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+          buf[(kFrags + nt) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
+        }
+      }
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float4 ml = buf[(kFrags + nt) * 32];
+          float fa[2], fb[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float ma = m[nt][x], mb = x ? ml.y : ml.x, mx = fmaxf(ma, mb);
+            // A side without a visible key holds zeros (or NaN, which stays).
+            fa[x] = ma == -INFINITY ? 1.0f : ex2_approx(ma - mx);
+            fb[x] = mb == -INFINITY ? 1.0f : ex2_approx(mb - mx);
+            m[nt][x] = mx;
+            l[nt][x] = l[nt][x] * fa[x] + (x ? ml.w : ml.z) * fb[x];
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const float4 y = buf[(nt * (D / 16) + i) * 32];
+            o[nt][i][0] = o[nt][i][0] * fa[0] + y.x * fb[0];
+            o[nt][i][1] = o[nt][i][1] * fa[1] + y.y * fb[1];
+            o[nt][i][2] = o[nt][i][2] * fa[0] + y.z * fb[0];
+            o[nt][i][3] = o[nt][i][3] * fa[1] + y.w * fb[1];
+          }
+        }
+      }
+      __syncthreads();
+    }
     const int64_t item0 = at_tile - cur.tile, item1 = item0 + cur.tiles.count;
     const bool whole = item0 >= t0 && item1 <= t1;
     const int slot_of_mine = item0 <= t0 ? 0 : 1;
-    // A thread holds d = 4 x .. 4 x + 3 of one head at a time.
-    auto write_out = [&](int h, int d, const float4 &v, float sum) {
-      if (h >= nh) return;
-      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-      uint2 w;
+    // Fragment i of a thread: d = r D / 8 + 2 i and + 1, columns 2t and 2t + 1
+    // of nt (x, z: the first column; y, w: the second), times 1 / sum.
+    auto write_out = [&](int nt, int i, const float4 &v, float sum0, float sum1) {
+      uint16_t *row = static_cast<uint16_t *>(p.O) + cur.b * p.o_stride +
+                      (int64_t)(h0 + nt * 8 + 2 * t) * D + r * (D / 8) + 2 * i;
+      const float i0 = sum0 != 0.0f ? 1.0f / sum0 : 0.0f, i1 = sum1 != 0.0f ? 1.0f / sum1 : 0.0f;
+      uint32_t a, b;
       if constexpr (BF16) {
-        __nv_bfloat162 a = __floats2bfloat162_rn(v.x * inv, v.y * inv), b = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-        w = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+        __nv_bfloat162 x = __floats2bfloat162_rn(v.x * i0, v.z * i0), y = __floats2bfloat162_rn(v.y * i1, v.w * i1);
+        a = *reinterpret_cast<uint32_t *>(&x);
+        b = *reinterpret_cast<uint32_t *>(&y);
       } else {
-        w = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+        a = pack_half2(v.x * i0, v.z * i0);
+        b = pack_half2(v.y * i1, v.w * i1);
       }
-      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.O) + cur.b * p.o_stride + (int64_t)(h0 + h) * D + d) = w;
+      if (nt * 8 + 2 * t < nh) *reinterpret_cast<uint32_t *>(row) = a;
+      if (nt * 8 + 2 * t + 1 < nh) *reinterpret_cast<uint32_t *>(row + D) = b;
     };
-    float *const my_slot = p.slots + ((size_t)blockIdx.x * 2 + slot_of_mine) * kSlotFloats;
-    for (int e = tid; e < NH * D / 4; e += kThreads) {
-      const int h = e / (D / 4), d = e % (D / 4) * 4;
-      float mm = -INFINITY;
+    float4 *const my_slot =
+        reinterpret_cast<float4 *>(p.slots + ((size_t)blockIdx.x * 2 + slot_of_mine) * kSlotFloats);
+    if (warp == 0) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, merge_m[w * NH + h]);
-      float sum = 0.0f;
-      float4 acc = make_float4(0, 0, 0, 0);
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = merge_m[w * NH + h];
-        const float f = mw == -INFINITY ? 0.0f : ex2_approx(mw - mm);
-        const float4 x = *reinterpret_cast<const float4 *>(merge_o + (w * NH + h) * S::kRow + d);
-        // A warp without a visible key has nothing to add (0, not 0 * NaN: its sum is 0 too).
-        acc.x += f * x.x;
-        acc.y += f * x.y;
-        acc.z += f * x.z;
-        acc.w += f * x.w;
-        sum += mw == -INFINITY ? merge_l[w * NH + h] : f * merge_l[w * NH + h];
-      }
-      if (whole) {
-        write_out(h, d, acc, sum);
-      } else {
-        __stcg(reinterpret_cast<float4 *>(my_slot + h * D + d), acc);
-        if (d == 0) {
-          __stcg(my_slot + NH * D + 2 * h, mm);
-          __stcg(my_slot + NH * D + 2 * h + 1, sum);
+        for (int i = 0; i < D / 16; ++i) {
+          const float4 v = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+          if (whole)
+            write_out(nt, i, v, l[nt][0], l[nt][1]);
+          else
+            __stcg(my_slot + (nt * (D / 16) + i) * 32 + lane, v);
+        }
+        // The maxima and sums of a slot: [column] pairs behind its fragments.
+        if (!whole && r == 0) {
+          float2 *ml = reinterpret_cast<float2 *>(my_slot + kFrags * 32) + nt * 8 + 2 * t;
+          __stcg(ml, make_float2(m[nt][0], l[nt][0]));
+          __stcg(ml + 1, make_float2(m[nt][1], l[nt][1]));
         }
       }
     }
@@ -563,57 +659,54 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(c
       // Joins the n parts a, a + step, ... into the output, or into part a's slot.
       auto join = [&](int a, int n, int step, bool to_out) {
         __threadfence();
-        float *w = merge_o;  // [n][NH] weights, then [NH] sums
+        float *w = merge;  // [n][NH] weights, [NH] sums, then [n][NH] parts' sums
         for (int e = tid; e < n * NH; e += kThreads) {
           const float *from = p.slots + slot_of(a + e / NH * step) * kSlotFloats + NH * D;
-          w[e] = __ldcg(from + 2 * (e % NH));
-          w[(n + 1) * NH + e] = __ldcg(from + 2 * (e % NH) + 1);
+          const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from) + e % NH);
+          w[e] = ml.x;
+          w[(n + 1) * NH + e] = ml.y;
         }
         __syncthreads();
+        float top = -INFINITY, sum = 0.0f;
         if (tid < NH) {
-          float mm = -INFINITY, sum = 0.0f;
-          for (int i = 0; i < n; ++i) mm = fmaxf(mm, w[i * NH + tid]);
+          for (int i = 0; i < n; ++i) top = fmaxf(top, w[i * NH + tid]);
           for (int i = 0; i < n; ++i) {
             const float mi = w[i * NH + tid];
-            // Of a part without a visible key: 0 and 0, or NaN.
-            const float f = mi == -INFINITY ? 1.0f : ex2_approx(mi - mm);
+            const float f = mi == -INFINITY ? 1.0f : ex2_approx(mi - top);
             w[i * NH + tid] = f;
             sum += f * w[(n + 1 + i) * NH + tid];
           }
           w[n * NH + tid] = sum;
-          merge_m[tid] = mm;
         }
         __syncthreads();
-        constexpr int kVecs = NH * D / 4 / kThreads;
+        constexpr int kVecs = kFrags * 32 / kThreads;
         float4 acc[kVecs];
 #pragma unroll
         for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(0, 0, 0, 0);
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
-          const float *from = p.slots + slot_of(a + i * step) * kSlotFloats;
+          const float4 *from = reinterpret_cast<const float4 *>(p.slots + slot_of(a + i * step) * kSlotFloats);
 #pragma unroll
           for (int x = 0; x < kVecs; ++x) {
-            const int e = tid + x * kThreads;
-            const float f = w[i * NH + e / (D / 4)];
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(from) + e);
-            acc[x] = make_float4(acc[x].x + f * v.x, acc[x].y + f * v.y, acc[x].z + f * v.z,
-                                 acc[x].w + f * v.w);
+            const int e = tid + x * kThreads, col = e / (D / 16 * 32) * 8 + 2 * t;
+            const float f0 = w[i * NH + col], f1 = w[i * NH + col + 1];
+            const float4 v = __ldcg(from + e);
+            acc[x] = make_float4(acc[x].x + f0 * v.x, acc[x].y + f1 * v.y, acc[x].z + f0 * v.z,
+                                 acc[x].w + f1 * v.w);
           }
         }
         if (!to_out) __syncthreads();  // every thread has read part a's slot
         float *to = p.slots + slot_of(a) * kSlotFloats;
 #pragma unroll
         for (int x = 0; x < kVecs; ++x) {
-          const int e = tid + x * kThreads, h = e / (D / 4);
+          const int e = tid + x * kThreads, nt = e / (D / 16 * 32), i = e / 32 % (D / 16);
           if (to_out)
-            write_out(h, e % (D / 4) * 4, acc[x], w[n * NH + h]);
+            write_out(nt, i, acc[x], w[n * NH + nt * 8 + 2 * t], w[n * NH + nt * 8 + 2 * t + 1]);
           else
             __stcg(reinterpret_cast<float4 *>(to) + e, acc[x]);
         }
-        if (!to_out && tid < NH) {
-          __stcg(to + NH * D + 2 * tid, merge_m[tid]);
-          __stcg(to + NH * D + 2 * tid + 1, w[n * NH + tid]);
-        }
+        if (!to_out && tid < NH)
+          __stcg(reinterpret_cast<float2 *>(to + NH * D) + tid, make_float2(top, sum));
       };
       // Counts this block in; true for the one that completes `of`.
       auto arrive = [&](unsigned *counter, int of) {
@@ -640,12 +733,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) kv8_attn_kernel(c
     cur.tile += n;
     if (at_tile < t1) next_item(cur, p);
   }
-  cp_async_wait<0>();
+  // Only a wait that ran out leaves copies behind: they get time to land.
+  for (int i = 0; !ok && i < kStages; ++i) {
+    mbar_wait(&full[stage], phase, 1000000000ull);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
 }
 
 template <int D, int NT, bool BF16>
 cudaError_t launch_typed(const AttnParams &p, cudaStream_t stream) {
-  constexpr int bytes = Smem<D>::template bytes<NT>();
+  constexpr int bytes = Smem<D, NT>::kBytes;
+  static_assert(blocks_per_sm(NT) * (bytes + 1024) <= 228 * 1024, "blocks per SM");
   static uint64_t configured = 0;  // devices whose smem attribute is set
   static std::mutex mu;
   int dev = 0;
@@ -661,6 +762,26 @@ cudaError_t launch_typed(const AttnParams &p, cudaStream_t stream) {
   }
   kv8_attn_kernel<D, NT, BF16><<<grid_blocks(NT), kThreads, bytes, stream>>>(p);
   return cudaGetLastError();
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Codes of K or V as (d, heads * page_size, pages), boxes of up to 32 tokens of a page.
+bool make_map(CUtensorMap *map, const vc_kv8_cache &c, void *codes) {
+  auto encode = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.heads * c.page_size,
+                              (cuuint64_t)c.num_pages};
+  const cuuint64_t strides[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_stride};
+  const cuuint32_t box[3] = {(cuuint32_t)c.head_dim, c.page_size < 32 ? 16u : 32u, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, codes, dims, strides, box, estr,
+                CU_TENSOR_MAP_INTERLEAVE_NONE,
+                c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace
@@ -681,12 +802,12 @@ cudaError_t launch_kv8_attn(const Kv8AttnArgs &a, cudaStream_t stream) {
   const int64_t tiles = (((int64_t)a.table_width << shift) + kTile - 1) / kTile + 1;
   if (tiles * a.B > INT32_MAX || tiles * c.heads * groups > INT32_MAX) return cudaErrorInvalidValue;
   float *slots = static_cast<float *>(a.workspace);
-  const AttnParams p{static_cast<const uint8_t *>(c.k), static_cast<const uint8_t *>(c.v),
-                     c.k_scale, c.v_scale, c.page_stride, c.scale_stride, a.q_stride, a.o_stride,
-                     a.Q, a.O, a.table, a.lens, slots,
-                     reinterpret_cast<Counters *>(slots + (size_t)grid_blocks(1) * 2 * kSlotFloats),
-                     a.B, c.num_pages, shift, c.heads, group, groups, a.table_width, a.window,
-                     a.sinks, a.scale_log2};
+  AttnParams p{{}, {}, c.k_scale, c.v_scale, c.scale_stride, a.q_stride, a.o_stride,
+               a.Q, a.O, a.table, a.lens, slots,
+               reinterpret_cast<Counters *>(slots + (size_t)grid_blocks(1) * 2 * kSlotFloats),
+               a.B, c.num_pages, shift, c.heads, group, groups, a.table_width, a.window,
+               a.sinks, a.scale_log2};
+  if (!make_map(&p.k, c, c.k) || !make_map(&p.v, c, c.v)) return cudaErrorInvalidValue;
   const bool bf16 = a.dtype == VC_DTYPE_BF16;
   if (c.head_dim == 64) {
     if (NT == 1) return bf16 ? launch_typed<64, 1, true>(p, stream) : launch_typed<64, 1, false>(p, stream);

@@ -1540,7 +1540,7 @@ VCError kv8_cache_checked(const vc_kv8_cache &c, const char *name) {
   if (c.head_dim != 64 && c.head_dim != 128) return VCError::InvalidValue;
   const int64_t page = (int64_t)c.heads * c.page_size * c.head_dim;
   if (page > INT32_MAX / 2 || c.page_stride < page || c.page_stride % 16 ||
-      c.page_stride > (int64_t)1 << 40 || c.scale_stride < c.heads ||
+      c.page_stride >= (int64_t)1 << 40 || c.scale_stride < c.heads ||
       c.scale_stride > (int64_t)1 << 40)
     return VCError::InvalidValue;
   const void *const p[4] = {c.k, c.v, c.k_scale, c.v_scale};
