@@ -166,6 +166,115 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
 }
 
+// Fragment i of a thread of the O^T product: d = r D / 8 + 2 i and + 1, columns
+// (query heads) 2t and 2t + 1 of nt (x, z: the first column; y, w: the second),
+// divided by the columns' sums into the output rows (of nh heads from `out` on).
+template <int D, bool BF16>
+__device__ __forceinline__ void write_fragment(uint16_t *out, int nh, int lane, int nt, int i,
+                                               const float4 &v, float sum0, float sum1) {
+  const int r = lane >> 2, t = lane & 3;
+  uint16_t *row = out + (nt * 8 + 2 * t) * D + r * (D / 8) + 2 * i;
+  // No visible key: zeros.
+  const float i0 = sum0 != 0.0f ? 1.0f / sum0 : 0.0f, i1 = sum1 != 0.0f ? 1.0f / sum1 : 0.0f;
+  uint32_t a, c;
+  if constexpr (BF16) {
+    __nv_bfloat162 x = __floats2bfloat162_rn(v.x * i0, v.z * i0), y = __floats2bfloat162_rn(v.y * i1, v.w * i1);
+    a = *reinterpret_cast<uint32_t *>(&x);
+    c = *reinterpret_cast<uint32_t *>(&y);
+  } else {
+    a = pack_half2(v.x * i0, v.z * i0);
+    c = pack_half2(v.y * i1, v.w * i1);
+  }
+  if (nt * 8 + 2 * t < nh) *reinterpret_cast<uint32_t *>(row) = a;
+  if (nt * 8 + 2 * t + 1 < nh) *reinterpret_cast<uint32_t *>(row + D) = c;
+}
+
+// Slot of part i of an item whose part 0 lies in block `first`: every later
+// part begins its block's range (slot 0).
+__device__ __forceinline__ size_t part_slot(int first, int first_slot, int i) {
+  return (size_t)(first + i) * 2 + (i ? 0 : first_slot);
+}
+
+// Joins the n parts a, a + step, ... of an item into the output rows, or (out
+// null) into part a's slot; 4 parts' loads are in flight at a time. Not inlined: its
+// registers are not the main loop's.
+template <int D, int NT, bool BF16>
+__device__ __noinline__ void join_parts(float *slots, int first, int first_slot, int a, int n,
+                                        int step, uint16_t *out, int nh) {
+  constexpr int kFrags = D / 16 * NT, kVecs = kFrags * 32 / kThreads;
+  constexpr int kBatch = 4;
+  const int tid = threadIdx.x, lane = tid & 31, t = lane & 3;
+  float4 acc[kVecs];
+  float mx[NT][2], sum[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    mx[nt][0] = mx[nt][1] = -INFINITY;
+    sum[nt][0] = sum[nt][1] = 0.0f;
+  }
+#pragma unroll
+  for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+    float4 v[kBatch][kVecs], ml[kBatch][NT];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      // Behind the last part: that one again, with weight 0.
+      const int part = a + min(i0 + i, n - 1) * step;
+      const float4 *from = reinterpret_cast<const float4 *>(slots + part_slot(first, first_slot, part) * kSlotFloats);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) ml[i][nt] = __ldcg(from + kFrags * 32 + nt * 4 + t);
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) v[i][x] = __ldcg(from + tid + x * kThreads);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float old0 = mx[nt][0], old1 = mx[nt][1];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        mx[nt][0] = fmaxf(mx[nt][0], ml[i][nt].x);
+        mx[nt][1] = fmaxf(mx[nt][1], ml[i][nt].z);
+      }
+      // A side without a visible key holds zeros (or NaN, which stays).
+      const float g0 = old0 == -INFINITY ? 1.0f : ex2_approx(old0 - mx[nt][0]);
+      const float g1 = old1 == -INFINITY ? 1.0f : ex2_approx(old1 - mx[nt][1]);
+      sum[nt][0] *= g0;
+      sum[nt][1] *= g1;
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x)
+        if (x * kThreads / (D / 16 * 32) == nt)
+          acc[x] = make_float4(acc[x].x * g0, acc[x].y * g1, acc[x].z * g0, acc[x].w * g1);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (i0 + i >= n) break;
+        const float f0 = ml[i][nt].x == -INFINITY ? 1.0f : ex2_approx(ml[i][nt].x - mx[nt][0]);
+        const float f1 = ml[i][nt].z == -INFINITY ? 1.0f : ex2_approx(ml[i][nt].z - mx[nt][1]);
+        sum[nt][0] += f0 * ml[i][nt].y;
+        sum[nt][1] += f1 * ml[i][nt].w;
+#pragma unroll
+        for (int x = 0; x < kVecs; ++x)
+          if (x * kThreads / (D / 16 * 32) == nt)
+            acc[x] = make_float4(acc[x].x + f0 * v[i][x].x, acc[x].y + f1 * v[i][x].y,
+                                 acc[x].z + f0 * v[i][x].z, acc[x].w + f1 * v[i][x].w);
+      }
+    }
+  }
+  if (!out) __syncthreads();  // every thread has read part a's slot
+  float4 *to = reinterpret_cast<float4 *>(slots + part_slot(first, first_slot, a) * kSlotFloats);
+#pragma unroll
+  for (int x = 0; x < kVecs; ++x) {
+    const int e = tid + x * kThreads, nt = x * kThreads / (D / 16 * 32);
+    if (out)
+      write_fragment<D, BF16>(out, nh, lane, nt, e / 32 % (D / 16), acc[x], sum[nt][0], sum[nt][1]);
+    else
+      __stcg(to + e, acc[x]);
+  }
+  if (!out && tid < 4) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      __stcg(to + kFrags * 32 + nt * 4 + t, make_float4(mx[nt][0], sum[nt][0], mx[nt][1], sum[nt][1]));
+  }
+}
+
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT))
 kv8_attn_kernel(const __grid_constant__ AttnParams p) {
@@ -185,6 +294,9 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     fence_barrier_init();
   }
   const int items = p.heads * p.groups;
+
+  grid_dependency_wait();
+  grid_launch_dependents();
 
   // ---- this block's range of tiles
   auto tiles_of = [&](int b) {
@@ -270,7 +382,7 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     const int i = pre.tile + lane;
     pages[0] = pages[1] = -1;
     scales[0] = scales[1] = scales[2] = scales[3] = 0.0f;
-    if (i >= pre.tiles.count || pre_t >= t1) return;
+    if (i >= pre.tiles.count || pre_t + lane >= t1) return;
     const int k0 = tile_key(pre.tiles, i, kTile) + warp * 32;
     const int32_t *row = p.table + (int64_t)pre.b * p.table_width;
     const int head = pre.item / p.groups;
@@ -278,60 +390,75 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (!any_visible(pre, k0 + 16 * h, 16)) continue;
-      pages[h] = __ldg(row + ((k0 + 16 * h) >> p.page_shift));
+      pages[h] = row[(k0 + 16 * h) >> p.page_shift];
       if (pages[h] < 0 || pages[h] >= p.num_pages) {
         pages[h] = -1;
         bad = true;
       } else {
-        scales[h] = __ldg(p.k_scale + pages[h] * p.scale_stride + head);
-        scales[2 + h] = __ldg(p.v_scale + pages[h] * p.scale_stride + head);
+        scales[h] = p.k_scale[pages[h] * p.scale_stride + head];
+        scales[2 + h] = p.v_scale[pages[h] * p.scale_stride + head];
       }
     }
     if (bad) record_error(kErrOutOfBounds);
   };
-  auto issue = [&](int stage) {
-    if (pre_t >= t1) return;
+  // One step's copies into a stage. The scales, which come a lookup later, go
+  // to `publish`, which also says how much the stage waits for.
+  auto copy = [&](int stage) {
+    uint32_t bytes = 0;
     if (lane == pre.tile - pages_at) {
       const int k0 = tile_key(pre.tiles, pre.tile, kTile) + warp * 32;
-      uint32_t mask = low_bits(pre.vis.len - k0) &
-                      (~low_bits(pre.vis.lo - k0) | low_bits(pre.vis.sink - k0));
-      if (pages[0] < 0) mask &= 0xffff0000u;
-      if (pages[1] < 0) mask &= 0x0000ffffu;
-      Meta &m = metas[stage];
-      m.k_scale[0] = scales[0];
-      m.k_scale[1] = scales[1];
-      m.v_scale[0] = scales[2];
-      m.v_scale[1] = scales[3];
-      m.mask = mask;
       uint8_t *at = ring + stage * S::kStage;
       const int row = ((pre.item / p.groups) << p.page_shift) + (k0 & ((1 << p.page_shift) - 1));
       if (two) {
-        const int n = (pages[0] >= 0) + (pages[1] >= 0);
-        mbar_arrive_expect_tx(&full[stage], n * 2 * S::kHalf);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (pages[h] >= 0) {
             tma_load_3d(at + h * S::kHalf, &p.k, 0, row, pages[h], &full[stage]);
             tma_load_3d(at + (2 + h) * S::kHalf, &p.v, 0, row, pages[h], &full[stage]);
+            bytes += 2 * S::kHalf;
           }
       } else {
         const int page = max(pages[0], pages[1]);
-        mbar_arrive_expect_tx(&full[stage], page >= 0 ? S::kStage : 0);
         if (page >= 0) {
           tma_load_3d(at, &p.k, 0, row, page, &full[stage]);
           tma_load_3d(at + 2 * S::kHalf, &p.v, 0, row, page, &full[stage]);
+          bytes = S::kStage;
         }
       }
     }
+    return bytes;
+  };
+  auto publish = [&](int stage, int tile, uint32_t bytes) {
+    if (lane != tile - pages_at) return;
+    const int k0 = tile_key(pre.tiles, tile, kTile) + warp * 32;
+    uint32_t mask = low_bits(pre.vis.len - k0) &
+                    (~low_bits(pre.vis.lo - k0) | low_bits(pre.vis.sink - k0));
+    if (pages[0] < 0) mask &= 0xffff0000u;
+    if (pages[1] < 0) mask &= 0x0000ffffu;
+    Meta &m = metas[stage];
+    m.k_scale[0] = scales[0];
+    m.k_scale[1] = scales[1];
+    m.v_scale[0] = scales[2];
+    m.v_scale[1] = scales[3];
+    m.mask = mask;
+    mbar_arrive_expect_tx(&full[stage], bytes);
+  };
+  auto advance = [&]() {
     ++pre_t;
     const bool turn = ++pre.tile == pre.tiles.count;
     if (turn && pre_t < t1) next_item(pre, p);
     if (turn || pre.tile - pages_at == 32) look_up();
   };
+  auto issue = [&](int stage) {
+    if (pre_t >= t1) return;
+    const uint32_t bytes = copy(stage);
+    publish(stage, pre.tile, bytes);
+    advance();
+  };
   __syncwarp();
   look_up();
 #pragma unroll 1
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
+  for (int s = 0; s < kStages; ++s) issue(s);
   uint32_t phase = 0;
   bool ok = true;
 
@@ -399,18 +526,21 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     if (n <= 0) break;
     for (int i = 0; i < n; ++i) {
       if (!ok) break;
-      __syncwarp();
-      issue(stage == 0 ? kStages - 1 : stage - 1);
       ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase));
       if (!ok) break;
       const uint32_t at = smem_u32(ring + stage * S::kStage);
       const uint4 sc = lds128(smem_u32(&metas[stage]));
       const uint32_t mask = metas[stage].mask;
+      const int mine = stage;
       if (++stage == kStages) {
         stage = 0;
         phase ^= 1;
       }
-      if (mask == 0) continue;  // uniform over the warp
+      if (mask == 0) {  // uniform over the warp
+        __syncwarp();
+        issue(mine);
+        continue;
+      }
       const float ks[2] = {__uint_as_float(sc.x), __uint_as_float(sc.y)};
       const float vs[2] = {__uint_as_float(sc.z), __uint_as_float(sc.w)};
 
@@ -550,6 +680,8 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
               mma16816(o[nt][2 * j + u], a0, a1, a2, a3, pb[h][nt][0], pb[h][nt][1]);
           }
       }
+      __syncwarp();
+      issue(mine);
     }
 
     // ---- the warps' results joined: 2 and 3 into 0 and 1, then 1 into 0, each
@@ -605,24 +737,7 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     const int64_t item0 = at_tile - cur.tile, item1 = item0 + cur.tiles.count;
     const bool whole = item0 >= t0 && item1 <= t1;
     const int slot_of_mine = item0 <= t0 ? 0 : 1;
-    // Fragment i of a thread: d = r D / 8 + 2 i and + 1, columns 2t and 2t + 1
-    // of nt (x, z: the first column; y, w: the second), times 1 / sum.
-    auto write_out = [&](int nt, int i, const float4 &v, float sum0, float sum1) {
-      uint16_t *row = static_cast<uint16_t *>(p.O) + cur.b * p.o_stride +
-                      (int64_t)(h0 + nt * 8 + 2 * t) * D + r * (D / 8) + 2 * i;
-      const float i0 = sum0 != 0.0f ? 1.0f / sum0 : 0.0f, i1 = sum1 != 0.0f ? 1.0f / sum1 : 0.0f;
-      uint32_t a, b;
-      if constexpr (BF16) {
-        __nv_bfloat162 x = __floats2bfloat162_rn(v.x * i0, v.z * i0), y = __floats2bfloat162_rn(v.y * i1, v.w * i1);
-        a = *reinterpret_cast<uint32_t *>(&x);
-        b = *reinterpret_cast<uint32_t *>(&y);
-      } else {
-        a = pack_half2(v.x * i0, v.z * i0);
-        b = pack_half2(v.y * i1, v.w * i1);
-      }
-      if (nt * 8 + 2 * t < nh) *reinterpret_cast<uint32_t *>(row) = a;
-      if (nt * 8 + 2 * t + 1 < nh) *reinterpret_cast<uint32_t *>(row + D) = b;
-    };
+    uint16_t *const out = static_cast<uint16_t *>(p.O) + cur.b * p.o_stride + (int64_t)h0 * D;
     float4 *const my_slot =
         reinterpret_cast<float4 *>(p.slots + ((size_t)blockIdx.x * 2 + slot_of_mine) * kSlotFloats);
     if (warp == 0) {
@@ -632,7 +747,7 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
         for (int i = 0; i < D / 16; ++i) {
           const float4 v = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
           if (whole)
-            write_out(nt, i, v, l[nt][0], l[nt][1]);
+            write_fragment<D, BF16>(out, nh, lane, nt, i, v, l[nt][0], l[nt][1]);
           else
             __stcg(my_slot + (nt * (D / 16) + i) * 32 + lane, v);
         }
@@ -655,65 +770,14 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       const int groups = (parts + size - 1) / size;
       // A part's slot: 1 where the item starts within the block's range.
       const int first_slot = split_start(total, blocks, first) < item0 ? 1 : 0;
-      auto slot_of = [&](int part) { return (size_t)(first + part) * 2 + (part ? 0 : first_slot); };
-      // Joins the n parts a, a + step, ... into the output, or into part a's slot.
-      auto join = [&](int a, int n, int step, bool to_out) {
-        __threadfence();
-        float *w = merge;  // [n][NH] weights, [NH] sums, then [n][NH] parts' sums
-        for (int e = tid; e < n * NH; e += kThreads) {
-          const float *from = p.slots + slot_of(a + e / NH * step) * kSlotFloats + NH * D;
-          const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from) + e % NH);
-          w[e] = ml.x;
-          w[(n + 1) * NH + e] = ml.y;
-        }
-        __syncthreads();
-        float top = -INFINITY, sum = 0.0f;
-        if (tid < NH) {
-          for (int i = 0; i < n; ++i) top = fmaxf(top, w[i * NH + tid]);
-          for (int i = 0; i < n; ++i) {
-            const float mi = w[i * NH + tid];
-            const float f = mi == -INFINITY ? 1.0f : ex2_approx(mi - top);
-            w[i * NH + tid] = f;
-            sum += f * w[(n + 1 + i) * NH + tid];
-          }
-          w[n * NH + tid] = sum;
-        }
-        __syncthreads();
-        constexpr int kVecs = kFrags * 32 / kThreads;
-        float4 acc[kVecs];
-#pragma unroll
-        for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-          const float4 *from = reinterpret_cast<const float4 *>(p.slots + slot_of(a + i * step) * kSlotFloats);
-#pragma unroll
-          for (int x = 0; x < kVecs; ++x) {
-            const int e = tid + x * kThreads, col = e / (D / 16 * 32) * 8 + 2 * t;
-            const float f0 = w[i * NH + col], f1 = w[i * NH + col + 1];
-            const float4 v = __ldcg(from + e);
-            acc[x] = make_float4(acc[x].x + f0 * v.x, acc[x].y + f1 * v.y, acc[x].z + f0 * v.z,
-                                 acc[x].w + f1 * v.w);
-          }
-        }
-        if (!to_out) __syncthreads();  // every thread has read part a's slot
-        float *to = p.slots + slot_of(a) * kSlotFloats;
-#pragma unroll
-        for (int x = 0; x < kVecs; ++x) {
-          const int e = tid + x * kThreads, nt = e / (D / 16 * 32), i = e / 32 % (D / 16);
-          if (to_out)
-            write_out(nt, i, acc[x], w[n * NH + nt * 8 + 2 * t], w[n * NH + nt * 8 + 2 * t + 1]);
-          else
-            __stcg(reinterpret_cast<float4 *>(to) + e, acc[x]);
-        }
-        if (!to_out && tid < NH)
-          __stcg(reinterpret_cast<float2 *>(to + NH * D) + tid, make_float2(top, sum));
-      };
-      // Counts this block in; true for the one that completes `of`.
+      // Counts this block in; true for the one that completes `of`. The block's
+      // stores are behind the barrier, and the one acquire-release addition
+      // orders them before, and the others' stores after, for all of it.
       auto arrive = [&](unsigned *counter, int of) {
-        __threadfence();
         __syncthreads();
         if (tid == 0) {
-          const unsigned before2 = atomicAdd(counter, 1u);
+          unsigned before2;
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before2) : "l"(counter) : "memory");
           sh_last = before2 + 1 == (unsigned)of;
           if (sh_last) *counter = 0;  // ready for the next call
         }
@@ -722,10 +786,11 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       };
       const int part = (int)blockIdx.x - first, g = part / size;
       const int ga = g * size, gb = min(ga + size, parts);
-      const size_t lead = slot_of(ga);
+      const size_t lead = part_slot(first, first_slot, ga);
       if (arrive(&p.counters[lead >> 1].group[lead & 1], gb - ga)) {
-        join(ga, gb - ga, 1, groups == 1);
-        if (groups > 1 && arrive(&p.counters[first].item, groups)) join(0, groups, size, true);
+        join_parts<D, NT, BF16>(p.slots, first, first_slot, ga, gb - ga, 1, groups == 1 ? out : nullptr, nh);
+        if (groups > 1 && arrive(&p.counters[first].item, groups))
+          join_parts<D, NT, BF16>(p.slots, first, first_slot, 0, groups, size, out, nh);
       }
     }
     __syncthreads();  // the merge buffer is free again
@@ -741,6 +806,24 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       phase ^= 1;
     }
   }
+}
+
+// A launch that may begin while the one before it ends (it waits for that
+// one's results itself).
+cudaError_t launch_dependent(const void *kernel, dim3 grid, int threads, int smem,
+                             const AttnParams &p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  void *args[] = {const_cast<AttnParams *>(&p)};
+  return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
 template <int D, int NT, bool BF16>
@@ -760,8 +843,8 @@ cudaError_t launch_typed(const AttnParams &p, cudaStream_t stream) {
       if (dev < 64) configured |= (1ull << dev);
     }
   }
-  kv8_attn_kernel<D, NT, BF16><<<grid_blocks(NT), kThreads, bytes, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(reinterpret_cast<const void *>(kv8_attn_kernel<D, NT, BF16>),
+                          dim3(grid_blocks(NT)), kThreads, bytes, p, stream);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
