@@ -269,7 +269,7 @@ int vc_flash_fwd(const void *Q, const void *K, const void *V, void *O, int BH,
  * keys j <= t with t - j < window or j < sinks; window 0: every j <= t.
  *   O[b][h][i] = sum_j p_j V[b][h / (Hq / Hkv)][j],
  *   p = softmax_2(scale_log2 * Q[b][h][i] . K[b][h / (Hq / Hkv)][j]).
- * A row that sees no key (t < 0) is zero. Hq is a multiple of Hkv, d 64 or
+ * A row that sees no key (t < 0) is zero. scale_log2 is positive, Hq is a multiple of Hkv, d 64 or
  * 128, dtype F16 or BF16. The strides (elements between batches, heads and
  * tokens, in this order; NULL: dense [B][H][N][d]) are multiples of 8, rows
  * contiguous and 16-byte aligned; along an axis of one entry they do not
@@ -320,7 +320,7 @@ int vc_kv8_append(const vc_kv8_cache *cache, const void *K, const void *V, int64
  * of 8, 16-byte aligned), F16 or BF16. The token of sequence b is its last,
  * at position lens[b] - 1, and sees the keys j < lens[b] with
  * j >= lens[b] - window (window 0: all) or j < sinks. lens[b] = 0 gives a zero
- * row. Hq is a multiple of cache->heads. Any positive scales within 2^-100 ..
+ * row. scale_log2 is positive, Hq a multiple of cache->heads. Any positive scales within 2^-100 ..
  * 2^119 (and 0) are taken. Several tokens of one sequence (a draft to verify)
  * are several rows with the same pages and growing lens.
  * workspace: vc_kv8_attn_workspace bytes, 256-byte aligned, zero before its

@@ -60,7 +60,8 @@ def _window(vc, **kw):
     dict(d=256), dict(dtype=0), dict(dtype=3), dict(window=-1), dict(sinks=-1), dict(lens=A + 1),
     dict(B=40000, Hq=2), dict(q_strides=[1024, 1024, 63]), dict(q_strides=[1024, 1024, 32]),
     dict(k_strides=[0, 0, 64]), dict(o_strides=[0, -1024, 64]), dict(v_strides=[0, 1024, 68]),
-    dict(q_strides=[0, 1 << 39, 64])])
+    dict(q_strides=[0, 1 << 39, 64]), dict(scale_log2=0.0), dict(scale_log2=-1.0),
+    dict(scale_log2=float("nan")), dict(scale_log2=float("inf")), dict(Nk=(1 << 30) + 8)])
 def test_window_refusals(vc, kw):
     assert _window(vc, **kw) == INVALID
 
@@ -93,7 +94,8 @@ def test_append_refusals(vc, kw):
     dict(Q=0), dict(O=0), dict(Q=A + 2), dict(table=0), dict(lens=0), dict(table_width=0), dict(B=-1),
     dict(Hq=0), dict(Hq=3), dict(window=-1), dict(sinks=-1), dict(dtype=0), dict(q_stride=192),
     dict(o_stride=260), dict(workspace=0), dict(workspace=A + 16), dict(B=65536),
-    dict(table_width=1 << 28)])
+    dict(table_width=1 << 28), dict(scale_log2=0.0), dict(scale_log2=-0.5),
+    dict(scale_log2=float("nan"))])
 def test_attn_refusals(vc, kw):
     a = dict(cache=_cache(vc), Q=A, O=A, table=A, table_width=4, lens=A, B=1, Hq=4, scale_log2=0.1,
              dtype=vc.Dtype.F16, workspace=A, workspace_bytes=1 << 30)

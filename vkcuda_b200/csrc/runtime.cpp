@@ -29,6 +29,7 @@
 
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <condition_variable>
 #include <cstdio>
 #include <cstdlib>
@@ -1491,6 +1492,9 @@ VCError ints_checked(const void *p, size_t n, const char *name) {
   return n * 4 > bytes_available(p) ? too_small(name) : VCError::Success;
 }
 
+// A score's factor: positive and finite (a maximum of the products is one of the scores).
+bool positive(float scale) { return scale > 0.0f && scale < INFINITY; }
+
 // Bytes that [B][H][N][d] 16-bit elements at these strides span.
 size_t span16(int B, int H, int N, int d, const int64_t *s) {
   return (size_t)((B - 1) * s[0] + (H - 1) * s[1] + (int64_t)(N - 1) * s[2] + d) * 2;
@@ -1503,6 +1507,7 @@ VCError flash_window_checked(vcb::FlashWindowArgs f, const int64_t *const stride
     return VCError::InvalidValue;
   if (f.dtype != VC_DTYPE_F16 && f.dtype != VC_DTYPE_BF16) return VCError::InvalidValue;
   if ((f.d != 64 && f.d != 128) || f.window < 0 || f.sinks < 0) return VCError::InvalidValue;
+  if (!positive(f.scale_log2) || f.Nq > (1 << 30) || f.Nk > (1 << 30)) return VCError::InvalidValue;
   if ((int64_t)f.B * f.Hq > 65535) return VCError::InvalidValue;
   int64_t *const to[4] = {f.sq, f.sk, f.sv, f.so};
   const void *const p[4] = {f.Q, f.K, f.V, f.O};
@@ -1593,7 +1598,7 @@ VCError kv8_attn_checked(const vcb::Kv8AttnArgs &a, size_t workspace_bytes, cuda
   if (!a.cache || a.B < 0 || a.Hq <= 0 || a.table_width <= 0 || a.window < 0 || a.sinks < 0)
     return VCError::InvalidValue;
   if (a.dtype != VC_DTYPE_F16 && a.dtype != VC_DTYPE_BF16) return VCError::InvalidValue;
-  if (a.B > 65535 || a.Hq > 65535) return VCError::InvalidValue;
+  if (!positive(a.scale_log2) || a.B > 65535 || a.Hq > 65535) return VCError::InvalidValue;
   VCError e = kv8_cache_checked(*a.cache, name);
   if (e != VCError::Success) return e;
   const vc_kv8_cache &c = *a.cache;
