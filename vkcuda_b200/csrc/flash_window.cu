@@ -39,7 +39,7 @@ namespace {
 constexpr int BQ = 128;    // query rows per tile (two tiles per CTA)
 constexpr int BKV = 128;   // keys per tile
 constexpr int kStages = 2;
-constexpr int kThreads = 320;  // 10 warps: 168 registers per thread at most
+constexpr int kThreads = 384;  // 12 warps of 168 registers, split 232 (softmax) / 40 (the rest)
 constexpr int kWgThreads = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows x 64 16-bit elements
@@ -180,136 +180,9 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
-  if (warp == 8) {
-    int issued = 0;
-    if (lane == 0 && total > 0) {
-      // ------------------------------------------------ TMA producer
-      tma_prefetch_desc(&p.q);
-      tma_prefetch_desc(&p.k);
-      tma_prefetch_desc(&p.v);
-      mbar_arrive_expect_tx(&bars->q_full, ((count0 > 0) + (count1 > 0)) * L::kTile);
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        if (w ? count1 > 0 : count0 > 0) {
-#pragma unroll
-          for (int c = 0; c < HD / 64; ++c)
-            tma_load_4d(smem + w * L::kTile + c * kBoxBytes, &p.q, c * 64, row0[w], head[w], b,
-                        &bars->q_full);
-        }
-      // Stage s = 0..total: V(s - 1) in its first tile slot (from s = 1), K(s)
-      // in its second (up to s = total - 1).
-      for (int s = 0; s <= total; ++s) {
-        const int st = s % kStages;
-        if (!mbar_wait(&bars->kv_empty[st], ((s / kStages) & 1) ^ 1)) break;
-        mbar_arrive_expect_tx(&bars->kv_full[st], ((s >= 1) + (s < total)) * L::kTile);
-        uint8_t *slot = smem + L::kRing + st * 2 * L::kTile;
-        const int kv = tile_of(s - 1) * BKV, kk = tile_of(s) * BKV;
-#pragma unroll
-        for (int c = 0; c < HD / 64; ++c) {
-          if (s >= 1)
-            tma_load_4d(slot + c * kBoxBytes, &p.v, c * 64, kv, kvh, b, &bars->kv_full[st]);
-          if (s < total)
-            tma_load_4d(slot + L::kTile + c * kBoxBytes, &p.k, c * 64, kk, kvh, b,
-                        &bars->kv_full[st]);
-        }
-        ++issued;
-      }
-    }
-    issued = __shfl_sync(0xffffffffu, issued, 0);
-    if (clean && issued == total + 1) {
-      // The last V tile, in stage `total`.
-      const int st = total % kStages;
-      bool ok = mbar_wait(&bars->kv_full[st], (total / kStages) & 1);
-      uint8_t *v = smem + L::kRing + st * 2 * L::kTile;
-      const int first = n - (hi - 1) * BKV;  // a 128-byte row per token and box
-      if (ok)
-        for (int i = lane; i < (BKV - first) * 8; i += 32)
-#pragma unroll
-          for (int c = 0; c < HD / 64; ++c)
-            *reinterpret_cast<uint4 *>(v + c * kBoxBytes + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->v_clean);
-    }
-    if (lane == 0 && total > 0) {
-      // No copy is in flight when the CTA ends.
-      mbar_wait(&bars->q_full, 0, 1000000000ull);
-      const int last = issued < kStages ? issued : kStages;
-      for (int i = 0; i < last; ++i) {
-        const int s = issued - 1 - i;
-        mbar_wait(&bars->kv_full[s % kStages], (s / kStages) & 1, 1000000000ull);
-      }
-    }
-  } else if (warp == 9) {
-    if (lane == 0 && total > 0) {
-      // ------------------------------------------------ MMA issuer
-      const uint32_t idesc_s = idesc_f16_f32(BQ, BKV, BF16, false, false);
-      const uint32_t idesc_o = idesc_f16_f32(BQ, HD, BF16, false, true);
-      // Descriptors are built once; a byte offset within the shared window is
-      // an add of (offset >> 4) to the descriptor's address field.
-      const uint64_t dq = smem_desc_sw128(smem_u32(smem), 16, 1024);
-      const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kRing), 16, 1024);
-      const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kRing), kBoxBytes, 1024);
-      const uint32_t dq_hi = (uint32_t)(dq >> 32), dk_hi = (uint32_t)(dk >> 32), dv_hi = (uint32_t)(dv >> 32);
-      // K(s) and V(s - 1) of stage s: second and first tile slot.
-      auto issue_s = [&](int w, int s) {
-        const uint32_t q_lo = (uint32_t)dq + w * (L::kTile >> 4);
-        const uint32_t k_lo = (uint32_t)dk + ((((s % kStages) * 2 + 1) * L::kTile) >> 4);
-        const uint32_t d_tmem = tmem + w * 128;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks / 4) * (kBoxBytes >> 4) + (ks % 4) * (32 >> 4);
-          mma_f16_ss_lohi(d_tmem, q_lo + off, dq_hi, k_lo + off, dk_hi, idesc_s, ks > 0 ? 1u : 0u);
-        }
-        mma_commit(&bars->s_full[w]);
-      };
-      int done[2] = {0, 0};  // PV products of each row tile so far
-      auto issue_pv = [&](int w, int s) {
-        const uint32_t v_lo = (uint32_t)dv + ((((s % kStages) * 2) * L::kTile) >> 4);
-        const uint32_t o_tmem = tmem + 256 + w * 128, p_tmem = tmem + w * 128;
-        constexpr int kSteps = (BKV / 16) / kHandoffs;  // K = 16 MMAs per part
-#pragma unroll
-        for (int h = 0; h < kHandoffs; ++h) {
-          if (!mbar_wait(&bars->p_full[w][h], done[w] & 1)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < kSteps; ++kk) {
-            const int ks = h * kSteps + kk;
-            mma_f16_ts_lohi(o_tmem, p_tmem + ks * 8, v_lo + ks * ((16 * 128) >> 4), dv_hi, idesc_o,
-                            (done[w] > 0 || ks > 0) ? 1u : 0u);
-          }
-        }
-        // Only the epilogue waits for O: one commit after the tile's last PV.
-        if (++done[w] == (w ? count1 : count0)) mma_commit(&bars->o_full[w]);
-        return true;
-      };
-      auto wait_stage = [&](int s) {
-        const bool ok = mbar_wait(&bars->kv_full[s % kStages], (s / kStages) & 1);
-        tc_fence_after();
-        return ok;
-      };
-      bool ok = mbar_wait(&bars->q_full, 0) && wait_stage(0);
-      if (ok) {
-        if (kt[0].has(tile_of(0))) issue_s(0, 0);
-        if (kt[1].has(tile_of(0))) issue_s(1, 0);
-        mma_commit(&bars->kv_empty[0]);
-      }
-      // Step u: stage u + 1 brings V(u) and K(u + 1); one commit after the
-      // step's last MMA releases it.
-      for (int u = 0; ok && u < total; ++u) {
-        const int s = u + 1;
-        if (!wait_stage(s)) break;
-        if (clean && s == total && !mbar_wait(&bars->v_clean, 0)) break;
-        const int t = tile_of(u), t_next = tile_of(s);
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (kt[w].has(t)) ok = ok && issue_pv(w, s);
-          if (ok && s < total && kt[w].has(t_next)) issue_s(w, s);
-        }
-        if (ok) mma_commit(&bars->kv_empty[s % kStages]);
-      }
-    }
-  } else {
+  // 256 x 232 + 128 x 40 = 384 x 168 registers.
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // -------------------------------------------------- softmax, warps 0..7
     const int w = warp >> 2;              // which query tile
     const int quad = warp & 3;            // TMEM lane quadrant
@@ -483,6 +356,138 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         }
       }
     }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  if (warp == 8) {
+    int issued = 0;
+    if (lane == 0 && total > 0) {
+      // ------------------------------------------------ TMA producer
+      tma_prefetch_desc(&p.q);
+      tma_prefetch_desc(&p.k);
+      tma_prefetch_desc(&p.v);
+      mbar_arrive_expect_tx(&bars->q_full, ((count0 > 0) + (count1 > 0)) * L::kTile);
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (w ? count1 > 0 : count0 > 0) {
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c)
+            tma_load_4d(smem + w * L::kTile + c * kBoxBytes, &p.q, c * 64, row0[w], head[w], b,
+                        &bars->q_full);
+        }
+      // Stage s = 0..total: V(s - 1) in its first tile slot (from s = 1), K(s)
+      // in its second (up to s = total - 1).
+      for (int s = 0; s <= total; ++s) {
+        const int st = s % kStages;
+        if (!mbar_wait(&bars->kv_empty[st], ((s / kStages) & 1) ^ 1)) break;
+        mbar_arrive_expect_tx(&bars->kv_full[st], ((s >= 1) + (s < total)) * L::kTile);
+        uint8_t *slot = smem + L::kRing + st * 2 * L::kTile;
+        const int kv = tile_of(s - 1) * BKV, kk = tile_of(s) * BKV;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) {
+          if (s >= 1)
+            tma_load_4d(slot + c * kBoxBytes, &p.v, c * 64, kv, kvh, b, &bars->kv_full[st]);
+          if (s < total)
+            tma_load_4d(slot + L::kTile + c * kBoxBytes, &p.k, c * 64, kk, kvh, b,
+                        &bars->kv_full[st]);
+        }
+        ++issued;
+      }
+    }
+    issued = __shfl_sync(0xffffffffu, issued, 0);
+    if (clean && issued == total + 1) {
+      // The last V tile, in stage `total`.
+      const int st = total % kStages;
+      bool ok = mbar_wait(&bars->kv_full[st], (total / kStages) & 1);
+      uint8_t *v = smem + L::kRing + st * 2 * L::kTile;
+      const int first = n - (hi - 1) * BKV;  // a 128-byte row per token and box
+      if (ok)
+        for (int i = lane; i < (BKV - first) * 8; i += 32)
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c)
+            *reinterpret_cast<uint4 *>(v + c * kBoxBytes + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->v_clean);
+    }
+    if (lane == 0 && total > 0) {
+      // No copy is in flight when the CTA ends.
+      mbar_wait(&bars->q_full, 0, 1000000000ull);
+      const int last = issued < kStages ? issued : kStages;
+      for (int i = 0; i < last; ++i) {
+        const int s = issued - 1 - i;
+        mbar_wait(&bars->kv_full[s % kStages], (s / kStages) & 1, 1000000000ull);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && total > 0) {
+      // ------------------------------------------------ MMA issuer
+      const uint32_t idesc_s = idesc_f16_f32(BQ, BKV, BF16, false, false);
+      const uint32_t idesc_o = idesc_f16_f32(BQ, HD, BF16, false, true);
+      // Descriptors are built once; a byte offset within the shared window is
+      // an add of (offset >> 4) to the descriptor's address field.
+      const uint64_t dq = smem_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kRing), 16, 1024);
+      const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kRing), kBoxBytes, 1024);
+      const uint32_t dq_hi = (uint32_t)(dq >> 32), dk_hi = (uint32_t)(dk >> 32), dv_hi = (uint32_t)(dv >> 32);
+      // K(s) and V(s - 1) of stage s: second and first tile slot.
+      auto issue_s = [&](int w, int s) {
+        const uint32_t q_lo = (uint32_t)dq + w * (L::kTile >> 4);
+        const uint32_t k_lo = (uint32_t)dk + ((((s % kStages) * 2 + 1) * L::kTile) >> 4);
+        const uint32_t d_tmem = tmem + w * 128;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t off = (ks / 4) * (kBoxBytes >> 4) + (ks % 4) * (32 >> 4);
+          mma_f16_ss_lohi(d_tmem, q_lo + off, dq_hi, k_lo + off, dk_hi, idesc_s, ks > 0 ? 1u : 0u);
+        }
+        mma_commit(&bars->s_full[w]);
+      };
+      int done[2] = {0, 0};  // PV products of each row tile so far
+      auto issue_pv = [&](int w, int s) {
+        const uint32_t v_lo = (uint32_t)dv + ((((s % kStages) * 2) * L::kTile) >> 4);
+        const uint32_t o_tmem = tmem + 256 + w * 128, p_tmem = tmem + w * 128;
+        constexpr int kSteps = (BKV / 16) / kHandoffs;  // K = 16 MMAs per part
+#pragma unroll
+        for (int h = 0; h < kHandoffs; ++h) {
+          if (!mbar_wait(&bars->p_full[w][h], done[w] & 1)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < kSteps; ++kk) {
+            const int ks = h * kSteps + kk;
+            mma_f16_ts_lohi(o_tmem, p_tmem + ks * 8, v_lo + ks * ((16 * 128) >> 4), dv_hi, idesc_o,
+                            (done[w] > 0 || ks > 0) ? 1u : 0u);
+          }
+        }
+        // Only the epilogue waits for O: one commit after the tile's last PV.
+        if (++done[w] == (w ? count1 : count0)) mma_commit(&bars->o_full[w]);
+        return true;
+      };
+      auto wait_stage = [&](int s) {
+        const bool ok = mbar_wait(&bars->kv_full[s % kStages], (s / kStages) & 1);
+        tc_fence_after();
+        return ok;
+      };
+      bool ok = mbar_wait(&bars->q_full, 0) && wait_stage(0);
+      if (ok) {
+        if (kt[0].has(tile_of(0))) issue_s(0, 0);
+        if (kt[1].has(tile_of(0))) issue_s(1, 0);
+        mma_commit(&bars->kv_empty[0]);
+      }
+      // Step u: stage u + 1 brings V(u) and K(u + 1); one commit after the
+      // step's last MMA releases it.
+      for (int u = 0; ok && u < total; ++u) {
+        const int s = u + 1;
+        if (!wait_stage(s)) break;
+        if (clean && s == total && !mbar_wait(&bars->v_clean, 0)) break;
+        const int t = tile_of(u), t_next = tile_of(s);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (kt[w].has(t)) ok = ok && issue_pv(w, s);
+          if (ok && s < total && kt[w].has(t_next)) issue_s(w, s);
+        }
+        if (ok) mma_commit(&bars->kv_empty[s % kStages]);
+      }
+    }
+  }
   }
 
   tc_fence_before();
