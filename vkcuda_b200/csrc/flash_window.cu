@@ -16,6 +16,14 @@
 // so that the softmax of one tile runs under the MMAs of the other, P handed
 // over in two halves, O rescaled when the maximum grows by more than 2^8.
 //
+// The CTAs are persistent: each takes its next pair of row tiles from the
+// grid's queue (cluster launch control), and the steps of one pair follow on
+// those of the last: the stage of a pair's last V brings the next pair's first
+// K, and its first S products are issued between the last PV products, so that
+// they run under the last softmax and the epilogue (set-up, fill and epilogue
+// of a fresh CTA took 7 us, of 21 to 69 in all). A scheduler warp takes the
+// pairs and writes what the other warps need into shared memory.
+//
 // What differs is which tiles meet. The row tiles of all query heads of a K/V
 // head, (rows 0..127 of its G heads, rows 128..255, ...), are paired in that
 // order, so that both tiles of a CTA mostly have the same rows, and with them
@@ -39,7 +47,7 @@ namespace {
 constexpr int BQ = 128;    // query rows per tile (two tiles per CTA)
 constexpr int BKV = 128;   // keys per tile
 constexpr int kStages = 2;
-constexpr int kThreads = 384;  // 12 warps of 168 registers, split 232 (softmax) / 40 (the rest)
+constexpr int kThreads = 384;  // 12 warps of 168 registers, split 216 (softmax) / 72 (the rest)
 constexpr int kWgThreads = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows x 64 16-bit elements
@@ -49,14 +57,39 @@ constexpr int kChunksPerHandoff = (BKV / 32) / kHandoffs;
 // K/V slices per ordering group (heaviest CTAs of every slice of a group first).
 constexpr int kOrderGroup = 8;
 
-struct __align__(8) WindowBarriers {
-  uint64_t q_full;
+// Key tiles of a tile of query rows: t < hi with t >= lo or t < sink.
+struct KeyTiles {
+  int sink, lo, hi;
+  __device__ __forceinline__ bool has(int t) const { return t < hi && (t >= lo || t < sink); }
+  __device__ __forceinline__ int count() const { return hi - lo + min(sink, lo); }
+};
+
+// A pair of row tiles of the query heads that share a K/V head, and the key
+// tiles of their union: [0, sink), then [lo, hi).
+struct Work {
+  int valid;                   // 0: the queue is empty
+  int b, kvh, n;               // n: tokens of the sequence
+  int row0[2], head[2], count[2], exists[2];
+  KeyTiles kt[2];
+  int lo, hi, sink, total;
+  int clean;                   // V's rows from n on are zeroed in the last tile
+  int chained;                 // K(0) shares the stage of the last pair's last V
+  int stage0, n_live, n_clean; // stage of K(0); pairs with keys, cleaned tiles before this one
+  __device__ __forceinline__ int tile_of(int u) const { return u < sink ? u : lo + (u - sink); }
+};
+
+struct __align__(16) WindowBarriers {
+  uint4 answer;  // of the grid's queue
+  Work work[2];
+  uint64_t answer_full;
+  uint64_t work_full[2], work_empty[2];
+  uint64_t q_full, q_empty;
   uint64_t kv_full[kStages];
   uint64_t kv_empty[kStages];
-  uint64_t v_clean;  // V rows behind the sequence's end are zeroed
+  uint64_t v_dirty, v_clean;  // the last V tile of a padded sequence is there; is zeroed
   uint64_t s_full[2];
   uint64_t p_full[2][kHandoffs];
-  uint64_t o_full[2];
+  uint64_t o_full[2], o_empty[2];
   uint32_t tmem_base;
 };
 
@@ -72,20 +105,73 @@ struct WindowSmem {
 };
 
 struct WindowParams {
-  CUtensorMap q, k, v, o;  // (d, tokens, heads, batch)
+  CUtensorMap q, k, v;  // (d, tokens, heads, batch)
   const int32_t *lens;
   uint16_t *O;
   int64_t so[3];
+  bool wide;  // O's rows begin on 32 bytes
   int Hq, Hkv, Nq, Nk, window, sinks;
   float scale_log2;
 };
 
-// Key tiles of a tile of query rows: t < hi with t >= lo or t < sink.
-struct KeyTiles {
-  int sink, lo, hi;
-  __device__ __forceinline__ bool has(int t) const { return t < hi && (t >= lo || t < sink); }
-  __device__ __forceinline__ int count() const { return hi - lo + min(sink, lo); }
-};
+// Order of the grid: groups of K/V slices, the last rows (with the most keys)
+// of every slice of a group first.
+__device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Work &k) {
+  const int lin = y * gridDim.x + x, per = kOrderGroup * gridDim.x;
+  const int g = lin / per, first = g * kOrderGroup;
+  const int gsz = min(kOrderGroup, (int)gridDim.y - first);
+  const int r = lin - g * per;
+  const int pair = gridDim.x - 1 - r / gsz, slice = first + r % gsz;
+  const int group = p.Hq / p.Hkv;
+  const int shift = p.Nk - p.Nq;  // position of row 0
+  const int b = slice / p.Hkv, kvh = slice - b * p.Hkv;
+  const int n = p.lens ? min(max(p.lens[b], 0), p.Nk) : p.Nk;
+  const int units = (p.Nq + BQ - 1) / BQ * group;
+  KeyTiles kt[2];
+  int count[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int unit = 2 * pair + w;
+    const int row0 = unit / group * BQ;
+    // Positions of the rows that are computed: the last one has the most keys.
+    const int t_first = max(row0 + shift, 0);
+    const int t_last = min(min(row0 + BQ, p.Nq) - 1 + shift, n - 1);
+    kt[w] = {0, 0, 0};
+    if (unit < units && t_last >= t_first) {
+      kt[w].hi = t_last / BKV + 1;
+      if (p.window > 0) {
+        kt[w].lo = max(t_first - p.window + 1, 0) / BKV;
+        kt[w].sink = (int)min(((int64_t)p.sinks + BKV - 1) / BKV, (int64_t)kt[w].lo);
+      }
+    }
+    count[w] = kt[w].count();
+    k.row0[w] = row0;
+    k.head[w] = kvh * group + unit % group;
+    k.exists[w] = unit < units;
+    k.count[w] = count[w];
+    k.kt[w] = kt[w];
+  }
+  const int lo = count[0] && count[1] ? min(kt[0].lo, kt[1].lo) : count[0] ? kt[0].lo : kt[1].lo;
+  const int hi = max(kt[0].hi, kt[1].hi);
+  const int sink = min(max(kt[0].sink, kt[1].sink), lo);
+  k.b = b;
+  k.kvh = kvh;
+  k.n = n;
+  k.lo = lo;
+  k.hi = hi;
+  k.sink = sink;
+  k.total = hi - lo + sink;
+  // V's rows behind the end of a padded sequence are zeroed in its last tile:
+  // their weights are 0, but 0 times what they hold may not be.
+  k.clean = n < p.Nk && hi > 0 && hi * BKV > n;
+}
+
+// 32 bytes, a whole sector, to a 32-byte aligned address.
+__device__ __forceinline__ void st_global_32(void *p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -109,65 +195,27 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // ---- which row tiles: groups of K/V slices, the last rows (with the most
-  // keys) of every slice of a group first.
-  int pair, slice;
-  {
-    const int64_t lin = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-    const int g = (int)(lin / ((int64_t)kOrderGroup * gridDim.x));
-    const int first = g * kOrderGroup;
-    const int gsz = min(kOrderGroup, (int)gridDim.y - first);
-    const int r = (int)(lin - (int64_t)g * kOrderGroup * gridDim.x);
-    pair = gridDim.x - 1 - r / gsz;
-    slice = first + r % gsz;
-  }
-  const int group = p.Hq / p.Hkv;
-  const int b = slice / p.Hkv, kvh = slice % p.Hkv;
-  const int shift = p.Nk - p.Nq;  // position of row 0
-  const int n = p.lens ? min(max(p.lens[b], 0), p.Nk) : p.Nk;
-  const int units = (p.Nq + BQ - 1) / BQ * group;
-  int row0[2], head[2];
-  KeyTiles kt[2];
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const int unit = 2 * pair + w;
-    row0[w] = unit / group * BQ;
-    head[w] = kvh * group + unit % group;
-    // Positions of the rows that are computed: the last one has the most keys.
-    const int t_first = max(row0[w] + shift, 0);
-    const int t_last = min(min(row0[w] + BQ, p.Nq) - 1 + shift, n - 1);
-    kt[w] = {0, 0, 0};
-    if (unit < units && t_last >= t_first) {
-      kt[w].hi = t_last / BKV + 1;
-      if (p.window > 0) {
-        kt[w].lo = max(t_first - p.window + 1, 0) / BKV;
-        kt[w].sink = (int)min(((int64_t)p.sinks + BKV - 1) / BKV, (int64_t)kt[w].lo);
-      }
-    }
-  }
-  const int count0 = kt[0].count(), count1 = kt[1].count();
-  // The union of both: tiles [0, sink), then [lo, hi).
-  const int lo = count0 && count1 ? min(kt[0].lo, kt[1].lo) : count0 ? kt[0].lo : kt[1].lo;
-  const int hi = max(kt[0].hi, kt[1].hi);
-  const int sink = min(max(kt[0].sink, kt[1].sink), lo);
-  const int total = hi - lo + sink;
-  auto tile_of = [&](int u) { return u < sink ? u : lo + (u - sink); };
-  // V's rows behind the end of a padded sequence are zeroed in its last tile:
-  // their weights are 0, but 0 times what they hold may not be.
-  const bool clean = n < p.Nk && hi > 0 && hi * BKV > n;
 
   if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->work_full[s], 1);
+      mbar_init(&bars->work_empty[s], 11);  // one per warp that reads it
+    }
+    mbar_init(&bars->answer_full, 1);
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&bars->kv_full[s], 1);
       mbar_init(&bars->kv_empty[s], 1);
     }
+    mbar_init(&bars->v_dirty, 1);
     mbar_init(&bars->v_clean, 1);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&bars->s_full[w], 1);
       for (int h = 0; h < kHandoffs; ++h)
         mbar_init(&bars->p_full[w][h], kWgThreads / 32);  // one per warp
       mbar_init(&bars->o_full[w], 1);
+      mbar_init(&bars->o_empty[w], kWgThreads / 32);
     }
     fence_barrier_init();
   }
@@ -179,10 +227,25 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  grid_dependency_wait();
+  grid_launch_dependents();
 
-  // 256 x 232 + 128 x 40 = 384 x 168 registers.
+  // The pairs, for every warp but the scheduler: `work` waits for pair `round`
+  // (false at the end of the queue, and on an error: then the others' waits
+  // run out too), `done` gives its slot back.
+  int round = 0;
+  auto wait_work = [&](int r) {
+    return __all_sync(0xffffffffu, mbar_wait(&bars->work_full[r & 1], (r >> 1) & 1));
+  };
+  auto done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->work_empty[round & 1]);
+    ++round;
+  };
+
+  // 256 x 216 + 128 x 72 = 384 x 168 registers.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // -------------------------------------------------- softmax, warps 0..7
     const int w = warp >> 2;              // which query tile
     const int quad = warp & 3;            // TMEM lane quadrant
@@ -190,304 +253,410 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t s_col = tmem + lane_off + w * 128;
     const uint32_t o_col = tmem + lane_off + 256 + w * 128;
-    const KeyTiles mine = w ? kt[1] : kt[0];
-    const int my_count = w ? count1 : count0;
-    const int my_row0 = w ? row0[1] : row0[0], my_head = w ? head[1] : head[0];
-    const int t_first = my_row0 + shift, t = t_first + row;  // positions
-    float m_run = -INFINITY;  // running max of scale_log2 * s
-    float l_run = 0.0f;
+    int n_s = 0, n_o = 0;  // S tiles and O tiles so far
     bool ok = true;
-    int j = 0;                // key tiles so far
-    for (int u = 0; u < total; ++u) {
-      const int tile = tile_of(u);
-      if (!mine.has(tile)) continue;
-      if (!mbar_wait(&bars->s_full[w], j & 1)) ok = false;
-      // Warp-uniform status: the TMEM accesses below are warp-collective.
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-      const int key0 = tile * BKV;
-      // The whole S row in registers with one wait.
-      uint32_t s[BKV / 32][32];
-      if constexpr (BF16) {
+    for (; wait_work(round) && bars->work[round & 1].valid; done()) {
+      const Work &k = bars->work[round & 1];
+      const KeyTiles mine = k.kt[w];
+      const int count = k.count[w], row0 = k.row0[w], head = k.head[w];
+      const int total = k.total, lo = k.lo, sink = k.sink, n = k.n;
+      const int t_first = row0 + p.Nk - p.Nq, t = t_first + row;  // positions
+      float m_run = -INFINITY;  // running max of scale_log2 * s
+      float l_run = 0.0f;
+      bool first = true;
+      for (int u = 0; u < total; ++u) {
+        const int tile = u < sink ? u : lo + (u - sink);
+        if (!mine.has(tile)) continue;
+        if (!mbar_wait(&bars->s_full[w], n_s & 1)) ok = false;
+        ++n_s;
+        // Warp-uniform status: the TMEM accesses below are warp-collective.
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        const int key0 = tile * BKV;
+        // The whole S row in registers with one wait.
+        uint32_t s[BKV / 32][32];
+        if constexpr (BF16) {
 #pragma unroll
-        for (int c = 0; c < BKV / 32; ++c) tmem_ld32(s_col + c * 32, s[c]);
-      } else {
-        tmem_ld128(s_col, *reinterpret_cast<uint32_t(*)[128]>(&s[0][0]));
-      }
-      tmem_ld_wait();
-      // Keys key0 + x of this row: hidden from x = end on, and below `begin`
-      // where they are no sinks (x >= keep).
-      if (key0 + BKV - 1 > t_first) {
-        const int end = t - key0 + 1;
-#pragma unroll
-        for (int c = 0; c < BKV / 32; ++c)
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (c * 32 + x >= end) s[c][x] = __float_as_uint(-INFINITY);
-      }
-      if (p.window > 0 && t_first + BQ - 1 - key0 >= p.window && key0 + BKV > p.sinks) {
-        const int begin = t - p.window + 1 - key0, keep = p.sinks - key0;
-#pragma unroll
-        for (int c = 0; c < BKV / 32; ++c)
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (c * 32 + x < begin && c * 32 + x >= keep) s[c][x] = __float_as_uint(-INFINITY);
-      }
-      // Row max: three-input max into 4 independent partial maxima.
-      float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < BKV / 32; ++c)
-#pragma unroll
-        for (int x = 0; x < 32; x += 2)
-          mxp[(x >> 1) & 3] = fmax3(mxp[(x >> 1) & 3], __uint_as_float(s[c][x]),
-                                    __uint_as_float(s[c][x + 1]));
-      const float mx = fmax3(fmaxf(mxp[0], mxp[1]), mxp[2], mxp[3]);
-      const float m_cand = fmaxf(m_run, mx * p.scale_log2);
-      const bool grow = m_cand > m_run + kRescaleThreshold;  // true where the first keys appear
-      // Warp-uniform decision (TMEM loads and stores are warp-collective).
-      const bool rescale = __any_sync(0xffffffffu, grow);
-      float alpha = 1.0f;
-      if (rescale) {
-        // A row may still have seen no key (then it stays at minus infinity).
-        if (m_cand != -INFINITY) alpha = ex2_approx(m_run - m_cand);
-        l_run *= alpha;
-        m_run = m_cand;
-      }
-      const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
-      const bool rescale_o = rescale && j > 0;  // warp-uniform
-      int handed = 0;                           // parts of P handed over
-      // P = exp2(scale_log2 * s - m) -> 16-bit pairs over S columns.
-      float lsp[4] = {0.f, 0.f, 0.f, 0.f};
-      const float neg_m = -m_use, scale = p.scale_log2;
-#pragma unroll
-      for (int c = 0; c < BKV / 32; ++c) {
-        uint32_t pr[16];
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          float x0, x1;
-          fma2(x0, x1, __uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1]), scale, scale,
-               neg_m, neg_m);
-          // Masked scores are -inf: the exponential returns exactly 0.
-          const float p0 = ex2_approx(x0);
-          const float p1 = ex2_approx(x1);
-          pr[x] = pack2<BF16>(p0, p1);
-          // bf16: the row sum adds the rounded values, so numerator and
-          // denominator use the same weights (with one dominant key the
-          // unrounded sum would leave that key's 2^-9 rounding in O).
-          const int a = 2 * (x & 1);
-          if constexpr (BF16)
-            add_bf16x2_to_f32(lsp[a], lsp[a + 1], pr[x]);
-          else
-            add2(lsp[a], lsp[a + 1], lsp[a], lsp[a + 1], p0, p1);
+          for (int c = 0; c < BKV / 32; ++c) tmem_ld32(s_col + c * 32, s[c]);
+        } else {
+          tmem_ld128(s_col, *reinterpret_cast<uint32_t(*)[128]>(&s[0][0]));
         }
-        tmem_st16(s_col + c * 16, pr);
-        if (rescale_o && c == 1) {
-          // S_w complete implies that O_w's products so far are: O_w is stable,
-          // and the next wait for the hand-offs below.
-#pragma unroll
-          for (int oc = 0; oc < HD / 32; ++oc) {
-            uint32_t o[32];
-            tmem_ld32(o_col + oc * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-            tmem_st32(o_col + oc * 32, o);
-          }
-        }
-        // Hand over every part whose P is complete (with an O rescale
-        // pending, not before it is done).
-        if ((c + 1) % kChunksPerHandoff == 0 && (!rescale_o || c >= 1)) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          const int upto = c / kChunksPerHandoff;
-          if (lane == 0)
-            for (int h = handed; h <= upto; ++h) mbar_arrive(&bars->p_full[w][h]);
-          handed = upto + 1;
-        }
-      }
-      l_run += (lsp[0] + lsp[1]) + (lsp[2] + lsp[3]);
-      ++j;
-      if (!ok) break;
-    }
-    // Epilogue: O / l -> 16-bit. Rows of the sequence (t < n); a row without a
-    // key is zero.
-    const bool exists = 2 * pair + w < units;
-    const bool mine_row = my_row0 + row < p.Nq && (!p.lens || t < n);
-    const float inv_l = l_run != 0.0f ? 1.0f / l_run : 0.0f;
-    const bool whole = !p.lens || t_first + BQ <= n;  // of the tile, but for rows past Nq
-    uint16_t *out = p.O + b * p.so[0] + my_head * p.so[1] + (int64_t)(my_row0 + row) * p.so[2];
-    if (exists && my_count == 0) {
-      if (mine_row && t < 0)
-        for (int c = 0; c < HD / 8; ++c) reinterpret_cast<uint4 *>(out)[c] = make_uint4(0, 0, 0, 0);
-    } else if (__all_sync(0xffffffffu, ok && exists && mbar_wait(&bars->o_full[w], 0))) {
-      tc_fence_after();
-      uint8_t *stage = smem + w * L::kTile;  // over this tile's Q
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(o_col + c * 32, o);
         tmem_ld_wait();
-        uint8_t *rowp = stage + (c / 2) * kBoxBytes + row * 128;
+        // Keys key0 + x of this row: hidden from x = end on, and below `begin`
+        // where they are no sinks (x >= keep).
+        if (key0 + BKV - 1 > t_first) {
+          const int end = t - key0 + 1;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint4 v;
-          v.x = pack2<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
-          v.y = pack2<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
-          v.z = pack2<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
-          v.w = pack2<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
-          if (whole) {
-            const int chunk = (c % 2) * 4 + q;
-            *reinterpret_cast<uint4 *>(rowp + ((chunk ^ (row & 7)) * 16)) = v;
-          } else if (mine_row) {
-            reinterpret_cast<uint4 *>(out)[c * 4 + q] = v;
+          for (int c = 0; c < BKV / 32; ++c)
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (c * 32 + x >= end) s[c][x] = __float_as_uint(-INFINITY);
+        }
+        if (p.window > 0 && t_first + BQ - 1 - key0 >= p.window && key0 + BKV > p.sinks) {
+          const int begin = t - p.window + 1 - key0, keep = p.sinks - key0;
+#pragma unroll
+          for (int c = 0; c < BKV / 32; ++c)
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (c * 32 + x < begin && c * 32 + x >= keep) s[c][x] = __float_as_uint(-INFINITY);
+        }
+        // Row max: three-input max into 4 independent partial maxima.
+        float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < BKV / 32; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; x += 2)
+            mxp[(x >> 1) & 3] = fmax3(mxp[(x >> 1) & 3], __uint_as_float(s[c][x]),
+                                      __uint_as_float(s[c][x + 1]));
+        const float mx = fmax3(fmaxf(mxp[0], mxp[1]), mxp[2], mxp[3]);
+        const float m_cand = fmaxf(m_run, mx * p.scale_log2);
+        const bool grow = m_cand > m_run + kRescaleThreshold;  // true where the first keys appear
+        // Warp-uniform decision (TMEM loads and stores are warp-collective).
+        const bool rescale = __any_sync(0xffffffffu, grow);
+        float alpha = 1.0f;
+        if (rescale) {
+          // A row may still have seen no key (then it stays at minus infinity).
+          if (m_cand != -INFINITY) alpha = ex2_approx(m_run - m_cand);
+          l_run *= alpha;
+          m_run = m_cand;
+        }
+        const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
+        const bool rescale_o = rescale && !first;  // warp-uniform
+        int handed = 0;                           // parts of P handed over
+        // P = exp2(scale_log2 * s - m) -> 16-bit pairs over S columns.
+        float lsp[4] = {0.f, 0.f, 0.f, 0.f};
+        const float neg_m = -m_use, scale = p.scale_log2;
+#pragma unroll
+        for (int c = 0; c < BKV / 32; ++c) {
+          uint32_t pr[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            float x0, x1;
+            fma2(x0, x1, __uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1]), scale, scale,
+                 neg_m, neg_m);
+            // Masked scores are -inf: the exponential returns exactly 0.
+            const float p0 = ex2_approx(x0);
+            const float p1 = ex2_approx(x1);
+            pr[x] = pack2<BF16>(p0, p1);
+            // bf16: the row sum adds the rounded values, so numerator and
+            // denominator use the same weights (with one dominant key the
+            // unrounded sum would leave that key's 2^-9 rounding in O).
+            const int a = 2 * (x & 1);
+            if constexpr (BF16)
+              add_bf16x2_to_f32(lsp[a], lsp[a + 1], pr[x]);
+            else
+              add2(lsp[a], lsp[a + 1], lsp[a], lsp[a + 1], p0, p1);
+          }
+          tmem_st16(s_col + c * 16, pr);
+          if (rescale_o && c == 1) {
+            // S_w complete implies that O_w's products so far are: O_w is stable,
+            // and the next wait for the hand-offs below.
+#pragma unroll
+            for (int oc = 0; oc < HD / 32; ++oc) {
+              uint32_t o[32];
+              tmem_ld32(o_col + oc * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              tmem_st32(o_col + oc * 32, o);
+            }
+          }
+          // Hand over every part whose P is complete (with an O rescale
+          // pending, not before it is done).
+          if ((c + 1) % kChunksPerHandoff == 0 && (!rescale_o || c >= 1)) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            const int upto = c / kChunksPerHandoff;
+            if (lane == 0)
+              for (int h = handed; h <= upto; ++h) mbar_arrive(&bars->p_full[w][h]);
+            handed = upto + 1;
           }
         }
+        l_run += (lsp[0] + lsp[1]) + (lsp[2] + lsp[3]);
+        first = false;
+        if (!ok) break;
       }
-      if (whole) {
-        fence_proxy_async_smem();
-        named_bar_sync(1 + w, kWgThreads);
-        if (quad == 0 && lane == 0) {
+      // O / l -> 16-bit. Rows of the sequence (t < n); a row without a key is
+      // zero.
+      const bool my_row = row0 + row < p.Nq && (!p.lens || t < n);
+      uint16_t *out = p.O + k.b * p.so[0] + head * p.so[1] + (int64_t)(row0 + row) * p.so[2];
+      if (count == 0) {
+        if (k.exists[w] && my_row && t < 0)
+          for (int c = 0; c < HD / 8; ++c) reinterpret_cast<uint4 *>(out)[c] = make_uint4(0, 0, 0, 0);
+      } else {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->o_full[w], n_o & 1));
+        ++n_o;
+        if (!ok) break;
+        tc_fence_after();
+        const float inv_l = l_run != 0.0f ? 1.0f / l_run : 0.0f;
+        uint32_t o[HD / 32][32];
 #pragma unroll
-          for (int c = 0; c < HD / 64; ++c)
-            tma_store_4d(&p.o, stage + c * kBoxBytes, c * 64, my_row0, my_head, b);
-          bulk_commit_group();
-          bulk_wait_group<0>();
+        for (int c = 0; c < HD / 32; ++c) tmem_ld32(o_col + c * 32, o[c]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->o_empty[w]);  // the next pair's products may begin
+        // A thread has a row: it writes it sector by sector.
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+          const uint32_t *f = &o[c / 2][c % 2 * 16];
+          uint32_t v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i] = pack2<BF16>(__uint_as_float(f[2 * i]) * inv_l, __uint_as_float(f[2 * i + 1]) * inv_l);
+          if (!my_row) continue;
+          if (p.wide) {
+            st_global_32(out + c * 16, v);
+          } else {
+            reinterpret_cast<uint4 *>(out)[2 * c] = make_uint4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<uint4 *>(out)[2 * c + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+          }
         }
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == 8) {
-    int issued = 0;
-    if (lane == 0 && total > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 10) {
+      // ------------------------------------------------ scheduler
+      if (lane == 0) {
+        int x = blockIdx.x, y = blockIdx.y;
+        int stage = 0, n_live = 0, n_clean = 0;
+        bool live = false;  // the last pair had keys
+        for (int r = 0;; ++r) {
+          if (!mbar_wait_idle(&bars->work_empty[r & 1], ((r >> 1) & 1) ^ 1)) break;
+          Work &k = bars->work[r & 1];
+          bool have = true;
+          if (r > 0) {
+            mbar_arrive_expect_tx(&bars->answer_full, 16);
+            steal_cta(&bars->answer, &bars->answer_full);
+            have = mbar_wait(&bars->answer_full, (r - 1) & 1) &&
+                   stolen_cta(smem_u32(&bars->answer), x, y);
+            fence_proxy_async_smem();  // read before the queue writes there again
+          }
+          k.valid = have;
+          if (have) {
+            work_of(p, x, y, k);
+            k.chained = live && k.total > 0;
+            live = k.total > 0;
+            if (live) {
+              // Its K(0) joins the last pair's last V, or begins a stage.
+              k.stage0 = k.chained ? stage - 1 : stage;
+              k.n_live = n_live++;
+              k.n_clean = n_clean;
+              n_clean += k.clean;
+              stage = k.stage0 + k.total + 1;
+            }
+          } else {
+            k.chained = 0;
+          }
+          mbar_arrive(&bars->work_full[r & 1]);
+          if (!have) break;
+        }
+      }
+    } else if (warp == 8) {
       // ------------------------------------------------ TMA producer
-      tma_prefetch_desc(&p.q);
-      tma_prefetch_desc(&p.k);
-      tma_prefetch_desc(&p.v);
-      mbar_arrive_expect_tx(&bars->q_full, ((count0 > 0) + (count1 > 0)) * L::kTile);
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        if (w ? count1 > 0 : count0 > 0) {
+      if (lane == 0) {
+        tma_prefetch_desc(&p.q);
+        tma_prefetch_desc(&p.k);
+        tma_prefetch_desc(&p.v);
+      }
+      bool ok = true;
+      // One stage: V of key tile tv of `kv`, K of key tile tk of `kk` (either may be absent).
+      auto load_stage = [&](int s, const Work *kv, int tv, const Work *kk, int tk) {
+        const int st = s % kStages;
+        if (!mbar_wait(&bars->kv_empty[st], ((s / kStages) & 1) ^ 1)) return false;
+        mbar_arrive_expect_tx(&bars->kv_full[st], ((kv != nullptr) + (kk != nullptr)) * L::kTile);
+        uint8_t *slot = smem + L::kRing + st * 2 * L::kTile;
+        if (kv) {
 #pragma unroll
           for (int c = 0; c < HD / 64; ++c)
-            tma_load_4d(smem + w * L::kTile + c * kBoxBytes, &p.q, c * 64, row0[w], head[w], b,
-                        &bars->q_full);
+            tma_load_4d(slot + c * kBoxBytes, &p.v, c * 64, tv * BKV, kv->kvh, kv->b, &bars->kv_full[st]);
         }
-      // Stage s = 0..total: V(s - 1) in its first tile slot (from s = 1), K(s)
-      // in its second (up to s = total - 1).
-      for (int s = 0; s <= total; ++s) {
-        const int st = s % kStages;
-        if (!mbar_wait(&bars->kv_empty[st], ((s / kStages) & 1) ^ 1)) break;
-        mbar_arrive_expect_tx(&bars->kv_full[st], ((s >= 1) + (s < total)) * L::kTile);
-        uint8_t *slot = smem + L::kRing + st * 2 * L::kTile;
-        const int kv = tile_of(s - 1) * BKV, kk = tile_of(s) * BKV;
+        if (kk) {
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) {
-          if (s >= 1)
-            tma_load_4d(slot + c * kBoxBytes, &p.v, c * 64, kv, kvh, b, &bars->kv_full[st]);
-          if (s < total)
-            tma_load_4d(slot + L::kTile + c * kBoxBytes, &p.k, c * 64, kk, kvh, b,
+          for (int c = 0; c < HD / 64; ++c)
+            tma_load_4d(slot + L::kTile + c * kBoxBytes, &p.k, c * 64, tk * BKV, kk->kvh, kk->b,
                         &bars->kv_full[st]);
         }
-        ++issued;
+        return true;
+      };
+      for (; ok && wait_work(round) && bars->work[round & 1].valid; done()) {
+        const Work &k = bars->work[round & 1], &next = bars->work[(round + 1) & 1];
+        if (k.total == 0) continue;
+        if (lane == 0) {
+          if (!k.chained) ok = load_stage(k.stage0, nullptr, 0, &k, k.tile_of(0));
+          ok = ok && mbar_wait(&bars->q_empty, (k.n_live & 1) ^ 1);
+          if (ok) {
+            mbar_arrive_expect_tx(&bars->q_full, ((k.count[0] > 0) + (k.count[1] > 0)) * L::kTile);
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+              if (k.count[w] > 0) {
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c)
+                  tma_load_4d(smem + w * L::kTile + c * kBoxBytes, &p.q, c * 64, k.row0[w], k.head[w],
+                              k.b, &bars->q_full);
+              }
+          }
+          for (int u = 0; ok && u + 1 < k.total; ++u)
+            ok = load_stage(k.stage0 + u + 1, &k, k.tile_of(u), &k, k.tile_of(u + 1));
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0) && wait_work(round + 1);
+        if (ok && lane == 0) {
+          const bool chain = next.valid && next.chained;
+          ok = load_stage(k.stage0 + k.total, &k, k.tile_of(k.total - 1), chain ? &next : nullptr,
+                          chain ? next.tile_of(0) : 0);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
       }
-    }
-    issued = __shfl_sync(0xffffffffu, issued, 0);
-    if (clean && issued == total + 1) {
-      // The last V tile, in stage `total`.
-      const int st = total % kStages;
-      bool ok = mbar_wait(&bars->kv_full[st], (total / kStages) & 1);
-      uint8_t *v = smem + L::kRing + st * 2 * L::kTile;
-      const int first = n - (hi - 1) * BKV;  // a 128-byte row per token and box
-      if (ok)
-        for (int i = lane; i < (BKV - first) * 8; i += 32)
+      // No copy is in flight when the CTA ends: the consumers have waited for
+      // every one, but for those behind an error, which get time to land.
+      if (!ok && lane == 0)
+        for (int i = 0; i < 2; ++i) {
+          mbar_wait(&bars->q_full, i, 100000000ull);
+          for (int st = 0; st < kStages; ++st) mbar_wait(&bars->kv_full[st], i, 100000000ull);
+        }
+    } else if (warp == 11) {
+      // ------------------------------------------------ V behind a sequence's end
+      auto idle_work = [&]() {
+        return __all_sync(0xffffffffu, mbar_wait_idle(&bars->work_full[round & 1], (round >> 1) & 1)) &&
+               bars->work[round & 1].valid;
+      };
+      for (bool ok = true; ok && idle_work(); done()) {
+        const Work &k = bars->work[round & 1];
+        if (!k.clean) continue;
+        // The issuer has seen the stage arrive; it stays until the issuer goes on
+        // (a stage's own barrier may be phases behind when this warp comes here).
+        const int s = k.stage0 + k.total, st = s % kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_dirty, k.n_clean & 1) &&
+                                         mbar_wait(&bars->kv_full[st], (s / kStages) & 1));
+        if (!ok) break;
+        // 128-byte rows of tokens in each box.
+        uint8_t *v = smem + L::kRing + st * 2 * L::kTile;
+        const int from = k.n - (k.hi - 1) * BKV;
+        for (int i = lane; i < (BKV - from) * 8; i += 32)
 #pragma unroll
           for (int c = 0; c < HD / 64; ++c)
-            *reinterpret_cast<uint4 *>(v + c * kBoxBytes + first * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->v_clean);
-    }
-    if (lane == 0 && total > 0) {
-      // No copy is in flight when the CTA ends.
-      mbar_wait(&bars->q_full, 0, 1000000000ull);
-      const int last = issued < kStages ? issued : kStages;
-      for (int i = 0; i < last; ++i) {
-        const int s = issued - 1 - i;
-        mbar_wait(&bars->kv_full[s % kStages], (s / kStages) & 1, 1000000000ull);
+            *reinterpret_cast<uint4 *>(v + c * kBoxBytes + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->v_clean);
       }
-    }
-  } else if (warp == 9) {
-    if (lane == 0 && total > 0) {
-      // ------------------------------------------------ MMA issuer
+    } else {
+      // ------------------------------------------------ MMA issuer, warp 9
+      // The whole warp runs the loop and one elected lane issues: what comes out
+      // of shared memory is broadcast, so that all of it is known to be alike in
+      // every lane and descriptors stay in uniform registers.
+      auto uni = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
       const uint32_t idesc_s = idesc_f16_f32(BQ, BKV, BF16, false, false);
       const uint32_t idesc_o = idesc_f16_f32(BQ, HD, BF16, false, true);
       // Descriptors are built once; a byte offset within the shared window is
       // an add of (offset >> 4) to the descriptor's address field.
       const uint64_t dq = smem_desc_sw128(smem_u32(smem), 16, 1024);
-      const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kRing), 16, 1024);
       const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kRing), kBoxBytes, 1024);
-      const uint32_t dq_hi = (uint32_t)(dq >> 32), dk_hi = (uint32_t)(dk >> 32), dv_hi = (uint32_t)(dv >> 32);
-      // K(s) and V(s - 1) of stage s: second and first tile slot.
-      auto issue_s = [&](int w, int s) {
-        const uint32_t q_lo = (uint32_t)dq + w * (L::kTile >> 4);
-        const uint32_t k_lo = (uint32_t)dk + ((((s % kStages) * 2 + 1) * L::kTile) >> 4);
-        const uint32_t d_tmem = tmem + w * 128;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks / 4) * (kBoxBytes >> 4) + (ks % 4) * (32 >> 4);
-          mma_f16_ss_lohi(d_tmem, q_lo + off, dq_hi, k_lo + off, dk_hi, idesc_s, ks > 0 ? 1u : 0u);
-        }
-        mma_commit(&bars->s_full[w]);
-      };
-      int done[2] = {0, 0};  // PV products of each row tile so far
-      auto issue_pv = [&](int w, int s) {
-        const uint32_t v_lo = (uint32_t)dv + ((((s % kStages) * 2) * L::kTile) >> 4);
-        const uint32_t o_tmem = tmem + 256 + w * 128, p_tmem = tmem + w * 128;
-        constexpr int kSteps = (BKV / 16) / kHandoffs;  // K = 16 MMAs per part
-#pragma unroll
-        for (int h = 0; h < kHandoffs; ++h) {
-          if (!mbar_wait(&bars->p_full[w][h], done[w] & 1)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < kSteps; ++kk) {
-            const int ks = h * kSteps + kk;
-            mma_f16_ts_lohi(o_tmem, p_tmem + ks * 8, v_lo + ks * ((16 * 128) >> 4), dv_hi, idesc_o,
-                            (done[w] > 0 || ks > 0) ? 1u : 0u);
-          }
-        }
-        // Only the epilogue waits for O: one commit after the tile's last PV.
-        if (++done[w] == (w ? count1 : count0)) mma_commit(&bars->o_full[w]);
-        return true;
-      };
-      auto wait_stage = [&](int s) {
-        const bool ok = mbar_wait(&bars->kv_full[s % kStages], (s / kStages) & 1);
-        tc_fence_after();
-        return ok;
-      };
-      bool ok = mbar_wait(&bars->q_full, 0) && wait_stage(0);
-      if (ok) {
-        if (kt[0].has(tile_of(0))) issue_s(0, 0);
-        if (kt[1].has(tile_of(0))) issue_s(1, 0);
-        mma_commit(&bars->kv_empty[0]);
-      }
-      // Step u: stage u + 1 brings V(u) and K(u + 1); one commit after the
-      // step's last MMA releases it.
-      for (int u = 0; ok && u < total; ++u) {
-        const int s = u + 1;
-        if (!wait_stage(s)) break;
-        if (clean && s == total && !mbar_wait(&bars->v_clean, 0)) break;
-        const int t = tile_of(u), t_next = tile_of(s);
+      const uint32_t dq_lo = (uint32_t)dq, dq_hi = (uint32_t)(dq >> 32);
+      const uint32_t dv_lo = (uint32_t)dv, dv_hi = (uint32_t)(dv >> 32);
+      static_assert(L::kRing == 2 * L::kTile, "Q0, Q1, then stages of V, K: one descriptor serves Q and K");
+      const uint32_t tm = uni(tmem);
+      // A wait that runs out is noted, and ends the loop at the end of its step
+      // (one vote a step, not one a wait).
+      bool fine = true;
+      auto wait = [&](uint64_t *bar, int parity) { fine = mbar_wait(bar, parity) && fine; };
+      int n_p[2] = {0, 0}, n_o[2] = {0, 0};  // P tiles and O tiles so far
+      bool ok = true;
+      for (; ok && wait_work(round) && uni(bars->work[round & 1].valid); done()) {
+        const Work &k = bars->work[round & 1], &next = bars->work[(round + 1) & 1];
+        const int total = uni(k.total);
+        if (total == 0) continue;
+        KeyTiles kt[2];
+        int left[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          if (kt[w].has(t)) ok = ok && issue_pv(w, s);
-          if (ok && s < total && kt[w].has(t_next)) issue_s(w, s);
+          kt[w] = {uni(k.kt[w].sink), uni(k.kt[w].lo), uni(k.kt[w].hi)};
+          left[w] = uni(k.count[w]);
         }
-        if (ok) mma_commit(&bars->kv_empty[s % kStages]);
+        const int lo = uni(k.lo), sink = uni(k.sink), stage0 = uni(k.stage0);
+        auto tile_of = [&](int u) { return u < sink ? u : lo + (u - sink); };
+        bool begun[2] = {false, false};
+        int u = uni(k.chained) ? 0 : -1;
+        if (u < 0) wait(&bars->q_full, uni(k.n_live) & 1);
+        // Step u in stage s = stage0 + u + 1: the products of V(u), and the scores
+        // of K(u + 1), which after the last step is the next pair's first. u = -1:
+        // scores only.
+#pragma unroll 1
+        for (; ok && u < total; ++u) {
+          const bool last = u + 1 == total;
+          const int tile = tile_of(u), after = tile_of(u + 1);
+          bool pv[2], sc[2];  // products and scores to issue
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            pv[w] = u >= 0 && kt[w].has(tile);
+            sc[w] = kt[w].has(after);
+          }
+          bool chain = false, q_free = u + 2 == total;
+          if (last) {
+            ok = wait_work(round + 1);
+            if (!ok) break;
+            chain = uni(next.valid && next.chained);
+            q_free = chain && uni(next.total) == 1;
+            const int t0 = next.tile_of(0);
+            sc[0] = uni(chain && next.kt[0].has(t0));
+            sc[1] = uni(chain && next.kt[1].has(t0));
+          }
+          const int s = stage0 + u + 1, st = s % kStages;
+          const uint32_t v_lo = dv_lo + (2 * st * L::kTile >> 4), k_lo = dq_lo + ((3 + 2 * st) * L::kTile >> 4);
+          wait(&bars->kv_full[st], (s / kStages) & 1);
+          if (last && uni(k.clean)) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->v_dirty);
+            __syncwarp();
+            wait(&bars->v_clean, uni(k.n_clean) & 1);
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (pv[w]) {
+              const uint32_t o_tmem = tm + 256 + w * 128, p_tmem = tm + w * 128;
+              constexpr int kSteps = (BKV / 16) / kHandoffs;  // K = 16 MMAs per part
+#pragma unroll
+              for (int h = 0; h < kHandoffs; ++h) {
+                wait(&bars->p_full[w][h], n_p[w] & 1);
+                // The last pair's O has been read.
+                if (h == 0 && !begun[w]) wait(&bars->o_empty[w], (n_o[w] & 1) ^ 1);
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < kSteps; ++kk) {
+                  const int ks = h * kSteps + kk;
+                  mma_f16_ts_lohi_warp(o_tmem, p_tmem + ks * 8, v_lo + ks * ((16 * 128) >> 4), dv_hi,
+                                       idesc_o, (begun[w] || ks > 0) ? 1u : 0u);
+                }
+              }
+              ++n_p[w];
+              begun[w] = true;
+              // Only the epilogue waits for O: one commit after the tile's last PV.
+              if (--left[w] == 0) {
+                mma_commit_warp(smem_u32(&bars->o_full[w]));
+                ++n_o[w];
+              }
+            }
+            if (w == 0 && chain) wait(&bars->q_full, uni(next.n_live) & 1);
+            if (sc[w]) {
+#pragma unroll
+              for (int ks = 0; ks < HD / 16; ++ks) {
+                const uint32_t off = (ks / 4) * (kBoxBytes >> 4) + (ks % 4) * (32 >> 4);
+                mma_f16_ss_lohi_warp(tm + w * 128, dq_lo + w * (L::kTile >> 4) + off, dq_hi, k_lo + off,
+                                     dq_hi, idesc_s, ks > 0 ? 1u : 0u);
+              }
+              mma_commit_warp(smem_u32(&bars->s_full[w]));
+            }
+          }
+          // Behind the last S of a pair, Q's tiles come free.
+          if (q_free) mma_commit_warp(smem_u32(&bars->q_empty));
+          mma_commit_warp(smem_u32(&bars->kv_empty[st]));
+          ok = __all_sync(0xffffffffu, fine);
+        }
       }
     }
-  }
   }
 
   tc_fence_before();
@@ -533,8 +702,17 @@ cudaError_t launch_typed(const WindowParams &p, dim3 grid, cudaStream_t stream) 
       if (dev < 64) configured |= (1ull << dev);
     }
   }
-  flash_window_kernel<HD, BF16><<<grid, kThreads, WindowSmem<HD>::kBytes, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = WindowSmem<HD>::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, flash_window_kernel<HD, BF16>, p);
 }
 
 }  // namespace
@@ -544,12 +722,15 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   WindowParams p;
   if (!make_map(&p.q, bf16, a.Q, a.B, a.Hq, a.Nq, a.d, a.sq) ||
       !make_map(&p.k, bf16, a.K, a.B, a.Hkv, a.Nk, a.d, a.sk) ||
-      !make_map(&p.v, bf16, a.V, a.B, a.Hkv, a.Nk, a.d, a.sv) ||
-      !make_map(&p.o, bf16, a.O, a.B, a.Hq, a.Nq, a.d, a.so))
+      !make_map(&p.v, bf16, a.V, a.B, a.Hkv, a.Nk, a.d, a.sv))
     return cudaErrorInvalidValue;
   p.lens = a.lens;
   p.O = static_cast<uint16_t *>(a.O);
-  for (int i = 0; i < 3; ++i) p.so[i] = a.so[i];
+  p.wide = reinterpret_cast<uintptr_t>(a.O) % 32 == 0;
+  for (int i = 0; i < 3; ++i) {
+    p.so[i] = a.so[i];
+    p.wide = p.wide && a.so[i] % 16 == 0;
+  }
   p.Hq = a.Hq;
   p.Hkv = a.Hkv;
   p.Nq = a.Nq;
@@ -558,7 +739,7 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   p.sinks = a.sinks;
   p.scale_log2 = a.scale_log2;
   const int64_t units = ((int64_t)a.Nq + BQ - 1) / BQ * (a.Hq / a.Hkv);
-  if (units > INT32_MAX / 2) return cudaErrorInvalidValue;
+  if ((units + 1) / 2 * a.B * a.Hkv > INT32_MAX / kOrderGroup) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((units + 1) / 2), a.B * a.Hkv);
   if (a.d == 64)
     return bf16 ? launch_typed<64, true>(p, grid, stream) : launch_typed<64, false>(p, grid, stream);

@@ -98,13 +98,34 @@ __device__ __forceinline__ bool mbar_test_nb(uint32_t bar_addr, uint32_t parity)
 // Wait for the completion of the barrier phase whose parity is `parity`.
 // Bounded by `limit_ns` of wall time; false (and an error recorded) on
 // timeout. `limit_ns` defaults to 4 s, far above any legitimate wait here.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
-                                          uint64_t limit_ns = 4000000000ull) {
-  const uint32_t addr = smem_u32(bar);
+__device__ __forceinline__ bool mbar_wait_at(uint32_t addr, uint32_t parity,
+                                             uint64_t limit_ns = 4000000000ull) {
   if (mbar_test_nb(addr, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   for (uint32_t spin = 1;; ++spin) {
     if (mbar_test_parity(addr, parity)) return true;
+    if ((spin & 255u) == 0u && global_timer_ns() - t0 > limit_ns) {
+      record_error(kErrWaitTimeout);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
+                                          uint64_t limit_ns = 4000000000ull) {
+  return mbar_wait_at(smem_u32(bar), parity, limit_ns);
+}
+
+// As mbar_wait, for a warp that waits long beside busy ones: it sleeps between
+// its tests, so that they take no issue slots from the others.
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t *bar, uint32_t parity,
+                                               uint64_t limit_ns = 4000000000ull) {
+  const uint32_t addr = smem_u32(bar);
+  if (mbar_test_nb(addr, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t spin = 1;; ++spin) {
+    __nanosleep(256);
+    if (mbar_test_nb(addr, parity)) return true;
     if ((spin & 255u) == 0u && global_timer_ns() - t0 > limit_ns) {
       record_error(kErrWaitTimeout);
       return false;
@@ -295,6 +316,35 @@ __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// Work stealing from the grid's own queue (cluster launch control): ask for a
+// CTA that has not started yet. The 16-byte answer arrives in shared memory
+// with completion on `bar`; a CTA that is given away does not start. After an
+// answer without one, no more may be asked for.
+__device__ __forceinline__ void steal_cta(void *smem_dst, uint64_t *bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(smem_dst)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The stolen CTA's index; false when none was left.
+__device__ __forceinline__ bool stolen_cta(uint32_t smem_addr, int &x, int &y) {
+  uint32_t ok, cx = 0, cy = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %2, r;\n\t}"
+      : "=r"(ok), "=r"(cx), "=r"(cy)
+      : "r"(smem_addr)
+      : "memory");
+  x = (int)cx;
+  y = (int)cy;
+  return ok != 0;
+}
+
 // ---------------------------------------------------------------- tcgen05
 // TMEM allocation: executed by one whole warp; the base address is written to
 // *dst_smem. ncols must be a power of two >= 32.
@@ -356,10 +406,44 @@ __device__ __forceinline__ void mma_f16_ts_lohi(uint32_t d_tmem, uint32_t a_tmem
 
 // Arrive (once) on `bar` when every tcgen05.mma issued so far by this thread
 // has completed.
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+__device__ __forceinline__ void mma_commit_at(uint32_t bar_addr) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) { mma_commit_at(smem_u32(bar)); }
+
+// The same, executed by a whole converged warp of which one elected lane issues
+// (operands that every lane computes alike stay warp-uniform).
+__device__ __forceinline__ void mma_f16_ss_lohi_warp(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
+                                                     uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                                     uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts_lohi_warp(uint32_t d_tmem, uint32_t a_tmem,
+                                                     uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                                     uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_warp(uint32_t bar_addr) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar_addr)
       : "memory");
 }
 
