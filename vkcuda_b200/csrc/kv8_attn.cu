@@ -196,7 +196,7 @@ __device__ __forceinline__ size_t part_slot(int first, int first_slot, int i) {
 }
 
 // Joins the n parts a, a + step, ... of an item into the output rows, or (out
-// null) into part a's slot; 4 parts' loads are in flight at a time. Not inlined: its
+// null) into part a's slot; the loads of 4 parts are in flight while 4 are added. Not inlined: its
 // registers are not the main loop's.
 template <int D, int NT, bool BF16>
 __device__ __noinline__ void join_parts(float *slots, int first, int first_slot, int a, int n,
@@ -213,9 +213,8 @@ __device__ __noinline__ void join_parts(float *slots, int first, int first_slot,
   }
 #pragma unroll
   for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(0, 0, 0, 0);
-#pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += kBatch) {
-    float4 v[kBatch][kVecs], ml[kBatch][NT];
+  float4 v[kBatch][kVecs], ml[kBatch][NT], v2[kBatch][kVecs], ml2[kBatch][NT];
+  auto load = [&](int i0, float4 (&v)[kBatch][kVecs], float4 (&ml)[kBatch][NT]) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       // Behind the last part: that one again, with weight 0.
@@ -226,6 +225,11 @@ __device__ __noinline__ void join_parts(float *slots, int first, int first_slot,
 #pragma unroll
       for (int x = 0; x < kVecs; ++x) v[i][x] = __ldcg(from + tid + x * kThreads);
     }
+  };
+  load(0, v, ml);
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+    if (i0 + kBatch < n) load(i0 + kBatch, v2, ml2);  // while this batch is added up
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float old0 = mx[nt][0], old1 = mx[nt][1];
@@ -256,6 +260,13 @@ __device__ __noinline__ void join_parts(float *slots, int first, int first_slot,
             acc[x] = make_float4(acc[x].x + f0 * v[i][x].x, acc[x].y + f1 * v[i][x].y,
                                  acc[x].z + f0 * v[i][x].z, acc[x].w + f1 * v[i][x].w);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) ml[i][nt] = ml2[i][nt];
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) v[i][x] = v2[i][x];
     }
   }
   if (!out) __syncthreads();  // every thread has read part a's slot

@@ -4,18 +4,20 @@
 // codes, with one fp32 scale per head, for K and V apart: x = code * scale.
 //
 // kv8_append_kernel: new 16-bit K/V tokens into the pages behind each
-// sequence's end. One block per (page touched, head, K or V): it loads the
-// page's new tokens once into registers, takes their largest magnitude,
-// raises the page's scale to it where needed (tokens already in the page are
-// then re-expressed at the new scale), rounds and stores. 2 bytes are read
-// and 1 written per element.
+// sequence's end. A block takes some of the (head, K or V) items of one page:
+// it loads an item's new tokens once into registers, takes their largest
+// magnitude, raises the page's scale to it where needed (tokens already in the
+// page are then re-expressed at the new scale), rounds and stores, while the
+// next item's tokens are on their way. 2 bytes are read and 1 written per
+// element: bound by HBM, once the pages are enough to fill the GPU.
 //
 // kv8_copy_kernel: whole pages src[i] -> dst[i], codes and scales, in every
-// layer with one launch; 16-byte copies, bound by HBM.
+// layer with one launch; bound by HBM.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <mutex>
 
 #include "internal.h"
 #include "kv8_index.h"
@@ -23,8 +25,6 @@
 
 namespace vcb {
 namespace {
-
-constexpr int kAppendThreads = 128;
 
 template <bool BF16>
 __device__ __forceinline__ float2 widen2(uint32_t p) {
@@ -56,18 +56,22 @@ struct AppendParams {
   const int32_t *table, *start, *cu;
   int32_t *lens_out;
   int num_pages, page_size, table_width, max_new, pages_per_seq, T;
+  int heads, per_block;  // (K or V, head) items of a block
 };
 
-// D / 8 threads per token (8 elements each), PASSES * 128 * 8 = page_size * D.
-template <int D, int PASSES, bool BF16>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendParams p) {
+// D / 8 threads per token (8 elements each), PASSES * THREADS * 8 = page_size * D.
+// Item i of a page: head i / 2 of K (i even) or V.
+template <int D, int THREADS, int PASSES, bool BF16>
+__global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kLanes = D / 8;                    // threads per token
-  constexpr int kRows = kAppendThreads / kLanes;   // tokens per pass
+  constexpr int kRows = THREADS / kLanes;          // tokens per pass
   const int b = blockIdx.x / p.pages_per_seq;
   const int pi = blockIdx.x % p.pages_per_seq;
-  const int head = blockIdx.y;
-  const int kv = blockIdx.z;
   const int P = p.page_size;
+  const int item0 = blockIdx.y * p.per_block, item1 = min(item0 + p.per_block, p.heads * 2);
+
+  grid_dependency_wait();
+  grid_launch_dependents();
 
   const int start = p.start[b];
   int64_t row0 = p.cu ? p.cu[b] : (int64_t)b * p.max_new;
@@ -80,7 +84,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     bad = true;
     n = start < room ? room - start : 0;
   }
-  const bool first_block = pi == 0 && head == 0 && kv == 0 && threadIdx.x == 0;
+  const bool first_block = pi == 0 && item0 == 0 && threadIdx.x == 0;
   if (first_block && p.lens_out) p.lens_out[b] = (int32_t)(bad && n == 0 ? (start < 0 ? 0 : start) : start + n);
   if (first_block && bad) record_error(kErrOutOfBounds);
   const int64_t pos0 = start > 0 ? start : 0;
@@ -94,97 +98,145 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     if (threadIdx.x == 0) record_error(kErrOutOfBounds);
     return;
   }
-  uint8_t *codes = p.codes[kv] + (int64_t)page * p.page_stride + (int64_t)head * P * D;
-  float *scale = p.scales[kv] + (int64_t)page * p.scale_stride + head;
   // Token of slot s: row0 + (page_idx * P + s - pos0).
   const int64_t tok0 = row0 + page_idx * P - pos0;
-  const char *src = static_cast<const char *>(p.src[kv]);
   const int lane = threadIdx.x % kLanes;
   const int row = threadIdx.x / kLanes;
-  const float old_raw = s0 > 0 ? *scale : 0.0f;
+  __shared__ float warp_max[2][THREADS / 32];
 
-  uint4 x[PASSES];
-  float amax = 0.0f;
+  auto load = [&](int item, uint4 (&x)[PASSES], float &old) {
+    const int kv = item & 1, head = item >> 1;
+    const char *src = static_cast<const char *>(p.src[kv]) +
+                      (tok0 * p.src_stride[kv] + (int64_t)head * D + lane * 8) * 2;
+    old = s0 > 0 ? p.scales[kv][(int64_t)page * p.scale_stride + head] : 0.0f;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int s = i * kRows + row;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (s >= s0 && s < s1)
-      x[i] = *reinterpret_cast<const uint4 *>(
-          src + ((tok0 + s) * p.src_stride[kv] + (int64_t)head * D + lane * 8) * 2);
-  }
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = widen2<BF16>(w[j]);
-      const float a = fabsf(f.x), c = fabsf(f.y);
-      // fmaxf passes NaN over; an infinity saturates instead of setting the scale.
-      if (a < INFINITY) amax = fmaxf(amax, a);
-      if (c < INFINITY) amax = fmaxf(amax, c);
+    for (int i = 0; i < PASSES; ++i) {
+      const int s = i * kRows + row;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (s >= s0 && s < s1) x[i] = __ldcs(reinterpret_cast<const uint4 *>(src + s * p.src_stride[kv] * 2));
     }
-  }
-  __shared__ float warp_max[kAppendThreads / 32];
+  };
+  uint4 x[PASSES], next[PASSES];
+  float old_raw, old_next = 0.0f;
+  load(item0, x, old_raw);
+#pragma unroll 1
+  for (int item = item0; item < item1; ++item) {
+    if (item + 1 < item1) load(item + 1, next, old_next);  // while this one is worked on
+    const int kv = item & 1, head = item >> 1;
+    uint8_t *codes = p.codes[kv] + (int64_t)page * p.page_stride + (int64_t)head * P * D;
+    float amax = 0.0f;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
-  __syncthreads();  // also: every thread has read the old scale
+    for (int i = 0; i < PASSES; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-  for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, warp_max[i]);
-
-  const float old = old_raw > 0.0f && old_raw < INFINITY ? old_raw : 0.0f;
-  const float sc = fmaxf(e4m3_block_scale(amax), old);
-  if (threadIdx.x == 0) *scale = sc;
-  if (s0 > 0 && sc != old) {
-    // The page's earlier tokens at the larger scale.
-    for (int s = row; s < s0; s += kRows) {
-      uint2 *at = reinterpret_cast<uint2 *>(codes + s * D + lane * 8);
-      const uint2 q = *at;
-      uint32_t out[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t w = j ? q.y : q.x;
-        const float2 a = from_e4m3x2(w & 0xFFFFu), c = from_e4m3x2(w >> 16);
-        out[j] = to_e4m3x2(a.x * old / sc, a.y * old / sc) |
-                 to_e4m3x2(c.x * old / sc, c.y * old / sc) << 16;
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = widen2<BF16>(w[j]);
+        const float a = fabsf(f.x), c = fabsf(f.y);
+        // fmaxf passes NaN over; an infinity saturates instead of setting the scale.
+        if (a < INFINITY) amax = fmaxf(amax, a);
+        if (c < INFINITY) amax = fmaxf(amax, c);
       }
-      *at = make_uint2(out[0], out[1]);
     }
-  }
-  // x / sc: a multiplication where sc is a power of two (exact), else the
-  // correctly rounded quotient.
-  const bool pow2 = (__float_as_uint(sc) & 0x7FFFFFu) == 0;
-  const float inv = 1.0f / sc;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int s = i * kRows + row;
-    if (s < s0 || s >= s1) continue;
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    uint32_t c[4];
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float *const top = warp_max[item & 1];  // the item before may still be read
+    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = amax;
+    __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = widen2<BF16>(w[j]);
-      c[j] = pow2 ? to_e4m3x2(f.x * inv, f.y * inv) : to_e4m3x2(f.x / sc, f.y / sc);
+    for (int i = 0; i < THREADS / 32; ++i) amax = fmaxf(amax, top[i]);
+
+    const float old = old_raw > 0.0f && old_raw < INFINITY ? old_raw : 0.0f;
+    const float sc = fmaxf(e4m3_block_scale(amax), old);
+    if (threadIdx.x == 0) p.scales[kv][(int64_t)page * p.scale_stride + head] = sc;
+    if (s0 > 0 && sc != old) {
+      // The page's earlier tokens at the larger scale.
+      for (int s = row; s < s0; s += kRows) {
+        uint2 *at = reinterpret_cast<uint2 *>(codes + s * D + lane * 8);
+        const uint2 q = *at;
+        uint32_t out[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t w = j ? q.y : q.x;
+          const float2 a = from_e4m3x2(w & 0xFFFFu), c = from_e4m3x2(w >> 16);
+          out[j] = to_e4m3x2(a.x * old / sc, a.y * old / sc) |
+                   to_e4m3x2(c.x * old / sc, c.y * old / sc) << 16;
+        }
+        *at = make_uint2(out[0], out[1]);
+      }
     }
-    *reinterpret_cast<uint2 *>(codes + s * D + lane * 8) =
-        make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    // x / sc: a multiplication where sc is a power of two (exact), else the
+    // correctly rounded quotient.
+    auto store = [&](auto scaled) {
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int s = i * kRows + row;
+        if (s < s0 || s >= s1) continue;
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = widen2<BF16>(w[j]);
+          c[j] = to_e4m3x2(scaled(f.x), scaled(f.y));
+        }
+        *reinterpret_cast<uint2 *>(codes + s * D + lane * 8) =
+            make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+      }
+    };
+    if ((__float_as_uint(sc) & 0x7FFFFFu) == 0) {
+      const float inv = 1.0f / sc;
+      store([&](float f) { return f * inv; });
+    } else {
+      store([&](float f) { return f / sc; });
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) x[i] = next[i];
+    old_raw = old_next;
   }
 }
 
-template <int D, int PASSES>
-void append_launch(const AppendParams &p, dim3 grid, bool bf16, cudaStream_t s) {
-  if (bf16)
-    kv8_append_kernel<D, PASSES, true><<<grid, kAppendThreads, 0, s>>>(p);
-  else
-    kv8_append_kernel<D, PASSES, false><<<grid, kAppendThreads, 0, s>>>(p);
+// A launch that may begin while the one before it ends (it waits for that
+// one's results itself).
+template <class P>
+cudaError_t launch_dependent(void (*kernel)(P), dim3 grid, int threads, int smem, const P &p,
+                             cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// At most 4 passes: 32 bytes of a token's tile in a thread's registers, and as
+// many of the next item's.
+template <int D, bool BF16>
+cudaError_t append_launch(const AppendParams &p, dim3 grid, cudaStream_t s) {
+  switch (p.page_size * D) {
+    case 1024: return launch_dependent(kv8_append_kernel<D, 128, 1, BF16>, grid, 128, 0, p, s);
+    case 2048: return launch_dependent(kv8_append_kernel<D, 128, 2, BF16>, grid, 128, 0, p, s);
+    case 4096: return launch_dependent(kv8_append_kernel<D, 128, 4, BF16>, grid, 128, 0, p, s);
+    case 8192: return launch_dependent(kv8_append_kernel<D, 256, 4, BF16>, grid, 256, 0, p, s);
+    case 16384: return launch_dependent(kv8_append_kernel<D, 512, 4, BF16>, grid, 512, 0, p, s);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 // ------------------------------------------------------------------ copy
-constexpr int kCopyThreads = 256;
-constexpr int kCopyVecs = 4;                                   // 16-byte loads in flight a thread
-constexpr int kCopyChunk = kCopyThreads * kCopyVecs * 16;      // bytes a block moves at a time
-constexpr int kCopyLayers = 64;                                // layers a launch takes
+constexpr int kCopyLayers = 64;          // layers a launch takes
+// Units of 16 KB, 2 blocks of 96 KB of ring per SM: 900 pages of 64 KB in 8
+// layers 156 us (6.07 TB/s), 8 pages of 128 KB in 16 layers 6.3 us. With 8 KB
+// units the one issuing thread is the bound (157 to 241 us); with 32 KB 152 us,
+// but 7.2 for the small case; 16-byte loads and stores by 8 blocks of 256
+// threads took 169 and 6.5 us.
+constexpr int kCopyChunk = 16384;        // bytes of a unit
+constexpr int kCopyStages = 6;           // of a block's ring
+constexpr int kCopyLag = 3;              // loads that run ahead of the stores
+constexpr int kCopyBlocksPerSm = 2;
 
 struct CopyParams {
   uint8_t *codes[kCopyLayers][2];
@@ -195,39 +247,85 @@ struct CopyParams {
   int num_pages, layers, heads, chunks, page_bytes;
 };
 
-__global__ void __launch_bounds__(kCopyThreads) kv8_copy_kernel(const __grid_constant__ CopyParams p) {
-  for (int64_t u = blockIdx.x; u < p.units; u += gridDim.x) {
-    const int chunk = (int)(u % p.chunks);
-    int64_t r = u / p.chunks;
-    const int kv = (int)(r & 1);
-    r >>= 1;
-    const int layer = (int)(r % p.layers);
-    const int64_t i = r / p.layers;
-    const int src = p.src[i], dst = p.dst[i];
-    if (src < 0 || src >= p.num_pages || dst < 0 || dst >= p.num_pages) {
-      if (threadIdx.x == 0) record_error(kErrOutOfBounds);
-      continue;
-    }
-    if (src == dst) continue;
-    const uint8_t *from = p.codes[layer][kv] + (int64_t)src * p.page_stride;
-    uint8_t *to = p.codes[layer][kv] + (int64_t)dst * p.page_stride;
-    uint4 v[kCopyVecs];
-    const int base = chunk * kCopyChunk + threadIdx.x * 16;
-#pragma unroll
-    for (int j = 0; j < kCopyVecs; ++j) {
-      const int at = base + j * kCopyThreads * 16;
-      if (at < p.page_bytes) v[j] = __ldcs(reinterpret_cast<const uint4 *>(from + at));
-    }
-#pragma unroll
-    for (int j = 0; j < kCopyVecs; ++j) {
-      const int at = base + j * kCopyThreads * 16;
-      if (at < p.page_bytes) __stcs(reinterpret_cast<uint4 *>(to + at), v[j]);
-    }
-    if (chunk == 0)
-      for (int h = threadIdx.x; h < p.heads; h += kCopyThreads)
-        p.scales[layer][kv][(int64_t)dst * p.scale_stride + h] =
-            p.scales[layer][kv][(int64_t)src * p.scale_stride + h];
+// One thread of warp 0 moves the codes through a ring of shared memory with
+// 1-D bulk copies, in and out again; warp 1 moves the scales.
+__global__ void __launch_bounds__(64) kv8_copy_kernel(const __grid_constant__ CopyParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kCopyStages];
+  __shared__ uint8_t *to[kCopyStages];  // of the loads on their way
+  __shared__ uint32_t bytes[kCopyStages];
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kCopyStages; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
   }
+  __syncthreads();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int64_t per_pair = (int64_t)p.layers * 2 * p.chunks;
+  if (threadIdx.x >= 32) {
+    // Scales: units of (pair, layer, K or V).
+    const int lane = threadIdx.x - 32;
+    for (int64_t u = blockIdx.x; u < p.units / p.chunks; u += gridDim.x) {
+      const int64_t i = u / (p.layers * 2);
+      const int which = (int)(u - i * (p.layers * 2));
+      const int src = p.src[i], dst = p.dst[i];
+      if (src < 0 || src >= p.num_pages || dst < 0 || dst >= p.num_pages) {
+        if (lane == 0) record_error(kErrOutOfBounds);
+        continue;
+      }
+      float *s = p.scales[which >> 1][which & 1];
+      if (src != dst)
+        for (int h = lane; h < p.heads; h += 32)
+          s[(int64_t)dst * p.scale_stride + h] = s[(int64_t)src * p.scale_stride + h];
+    }
+    return;
+  }
+  if (threadIdx.x != 0) return;
+  // The unit's place; its page numbers are fetched a unit ahead.
+  int64_t u = blockIdx.x;
+  int src = -1, dst = -1;
+  if (u < p.units) {
+    src = p.src[u / per_pair];
+    dst = p.dst[u / per_pair];
+  }
+  int loaded = 0, stored = 0;
+  bool ok = true;
+  auto store = [&]() {
+    const int st = stored % kCopyStages;
+    ok = mbar_wait(&full[st], (stored / kCopyStages) & 1);
+    if (!ok) return;
+    bulk_store_1d(to[st], ring + st * kCopyChunk, bytes[st]);
+    bulk_commit_group();
+    ++stored;
+  };
+  for (; ok && u < p.units;) {
+    const int64_t r = u % per_pair;
+    const int which = (int)(r / p.chunks), chunk = (int)(r % p.chunks);
+    const bool good = src >= 0 && src < p.num_pages && dst >= 0 && dst < p.num_pages && src != dst;
+    uint8_t *base = p.codes[which >> 1][which & 1] + (int64_t)chunk * kCopyChunk;
+    uint8_t *from = base + (int64_t)src * p.page_stride, *dest = base + (int64_t)dst * p.page_stride;
+    u += gridDim.x;
+    if (u < p.units) {
+      src = p.src[u / per_pair];
+      dst = p.dst[u / per_pair];
+    }
+    if (!good) continue;  // out of range (the scales' warp reports it), or onto itself
+    if (loaded >= kCopyLag) store();
+    if (!ok) break;
+    // The stage's last store, kCopyStages loads ago, has been read.
+    bulk_wait_group_read<kCopyStages - kCopyLag>();
+    const int st = loaded % kCopyStages;
+    bytes[st] = min(kCopyChunk, p.page_bytes - chunk * kCopyChunk);
+    to[st] = dest;
+    mbar_arrive_expect_tx(&full[st], bytes[st]);
+    bulk_load_1d(ring + st * kCopyChunk, from, bytes[st], &full[st]);
+    ++loaded;
+  }
+  while (ok && stored < loaded) store();
+  // After a wait that ran out, copies on their way get time to land.
+  for (; !ok && stored < loaded; ++stored)
+    mbar_wait(&full[stored % kCopyStages], (stored / kCopyStages) & 1, 1000000000ull);
+  bulk_wait_group<0>();
 }
 
 }  // namespace
@@ -258,27 +356,17 @@ cudaError_t launch_kv8_append(const Kv8AppendArgs &a, cudaStream_t stream) {
   const int64_t pages = ((int64_t)a.max_new - 1 + c.page_size - 1) / c.page_size + 1;
   if (pages * a.B > INT32_MAX) return cudaErrorInvalidValue;
   p.pages_per_seq = (int)pages;
-  const dim3 grid((unsigned)(pages * a.B), c.heads, 2);
+  // All items of a page in one block hide the look-up of lengths and page
+  // behind more work (37k tokens, 8 heads: 50 us against 67 with one item a
+  // block); where that would leave SMs idle, as for single tokens, fewer.
+  const int64_t items = (int64_t)c.heads * 2, blocks = (int64_t)sm_count_current() * 8;
+  p.heads = c.heads;
+  p.per_block = (int)(pages * a.B >= blocks ? items : (pages * a.B * items + blocks - 1) / blocks);
+  const dim3 grid((unsigned)(pages * a.B), (unsigned)((items + p.per_block - 1) / p.per_block));
   const bool bf16 = a.dtype == VC_DTYPE_BF16;
-  const int passes = c.page_size * c.head_dim / (kAppendThreads * 8);
-  if (c.head_dim == 64) {
-    switch (passes) {
-      case 1: append_launch<64, 1>(p, grid, bf16, stream); break;
-      case 2: append_launch<64, 2>(p, grid, bf16, stream); break;
-      case 4: append_launch<64, 4>(p, grid, bf16, stream); break;
-      case 8: append_launch<64, 8>(p, grid, bf16, stream); break;
-      default: return cudaErrorInvalidValue;
-    }
-  } else {
-    switch (passes) {
-      case 2: append_launch<128, 2>(p, grid, bf16, stream); break;
-      case 4: append_launch<128, 4>(p, grid, bf16, stream); break;
-      case 8: append_launch<128, 8>(p, grid, bf16, stream); break;
-      case 16: append_launch<128, 16>(p, grid, bf16, stream); break;
-      default: return cudaErrorInvalidValue;
-    }
-  }
-  return cudaGetLastError();
+  if (c.head_dim == 64)
+    return bf16 ? append_launch<64, true>(p, grid, stream) : append_launch<64, false>(p, grid, stream);
+  return bf16 ? append_launch<128, true>(p, grid, stream) : append_launch<128, false>(p, grid, stream);
 }
 
 cudaError_t launch_kv8_copy(const vc_kv8_cache *layers, int n_layers, const int32_t *src,
@@ -303,10 +391,22 @@ cudaError_t launch_kv8_copy(const vc_kv8_cache *layers, int n_layers, const int3
     p.page_bytes = c.heads * c.page_size * c.head_dim;
     p.chunks = (p.page_bytes + kCopyChunk - 1) / kCopyChunk;
     p.units = (int64_t)n * p.layers * 2 * p.chunks;
-    const int64_t most = (int64_t)sm_count_current() * 8;
+    const int64_t most = (int64_t)sm_count_current() * kCopyBlocksPerSm;
     const unsigned grid = (unsigned)(p.units < most ? p.units : most);
-    kv8_copy_kernel<<<grid, kCopyThreads, 0, stream>>>(p);
-    cudaError_t e = cudaGetLastError();
+    constexpr int bytes = kCopyStages * kCopyChunk;
+    static uint64_t configured = 0;  // devices whose smem attribute is set
+    static std::mutex mu;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    {
+      std::lock_guard<std::mutex> lk(mu);
+      if (dev >= 64 || !(configured & (1ull << dev))) {
+        cudaError_t e = cudaFuncSetAttribute(kv8_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) configured |= (1ull << dev);
+      }
+    }
+    cudaError_t e = launch_dependent(kv8_copy_kernel, dim3(grid), 64, bytes, p, stream);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
