@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
   const int64_t tok0 = row0 + page_idx * P - pos0;
   const int lane = threadIdx.x % kLanes;
   const int row = threadIdx.x / kLanes;
-  __shared__ float warp_max[2][THREADS / 32];
+  __shared__ uint32_t warp_max[2][THREADS / 32];
 
   auto load = [&](int item, uint4 (&x)[PASSES], float &old) {
     const int kv = item & 1, head = item >> 1;
@@ -124,26 +124,44 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
     if (item + 1 < item1) load(item + 1, next, old_next);  // while this one is worked on
     const int kv = item & 1, head = item >> 1;
     uint8_t *codes = p.codes[kv] + (int64_t)page * p.page_stride + (int64_t)head * P * D;
-    float amax = 0.0f;
+    // Magnitudes of 16-bit floats order as their bits do, infinity and NaN on
+    // top: one packed maximum per pair, and a second look only where it meets
+    // one of those (an infinity saturates instead of setting the scale).
+    constexpr uint32_t kInf = BF16 ? 0x7F80u : 0x7C00u;
+    uint32_t top2 = 0;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = widen2<BF16>(w[j]);
-        const float a = fabsf(f.x), c = fabsf(f.y);
-        // fmaxf passes NaN over; an infinity saturates instead of setting the scale.
-        if (a < INFINITY) amax = fmaxf(amax, a);
-        if (c < INFINITY) amax = fmaxf(amax, c);
-      }
+      top2 = __vmaxu2(top2, x[i].x & 0x7FFF7FFFu);
+      top2 = __vmaxu2(top2, x[i].y & 0x7FFF7FFFu);
+      top2 = __vmaxu2(top2, x[i].z & 0x7FFF7FFFu);
+      top2 = __vmaxu2(top2, x[i].w & 0x7FFF7FFFu);
     }
+    uint32_t *const tops = warp_max[item & 1];  // the item before may still be read
+    auto block_max = [&](uint32_t v) {
+      v = __reduce_max_sync(0xffffffffu, v);
+      if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = v;
+      __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float *const top = warp_max[item & 1];  // the item before may still be read
-    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = amax;
-    __syncthreads();  // also: every thread has read the old scale
+      for (int i = 0; i < THREADS / 32; ++i) v = max(v, tops[i]);
+      return v;
+    };
+    uint32_t top = block_max(max(top2 & 0xFFFFu, top2 >> 16));
+    if (top >= kInf) {
+      uint32_t finite = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) amax = fmaxf(amax, top[i]);
+      for (int i = 0; i < PASSES; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = w[j] & 0x7FFFu, hi = w[j] >> 16 & 0x7FFFu;
+          if (lo < kInf) finite = max(finite, lo);
+          if (hi < kInf) finite = max(finite, hi);
+        }
+      }
+      __syncthreads();  // every thread has read the first maxima
+      top = block_max(finite);
+    }
+    const float amax = widen2<BF16>(top).x;
 
     const float old = old_raw > 0.0f && old_raw < INFINITY ? old_raw : 0.0f;
     const float sc = fmaxf(e4m3_block_scale(amax), old);
@@ -165,28 +183,37 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
       }
     }
     // x / sc: a multiplication where sc is a power of two (exact), else the
-    // correctly rounded quotient.
-    auto store = [&](auto scaled) {
+    // correctly rounded quotient. fp16 pairs multiply and convert packed where
+    // 1 / sc is an fp16 number: what underflows there is zero in e4m3 as well.
+    auto store = [&](auto codes_of) {
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int s = i * kRows + row;
         if (s < s0 || s >= s1) continue;
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        uint32_t c[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = widen2<BF16>(w[j]);
-          c[j] = to_e4m3x2(scaled(f.x), scaled(f.y));
-        }
         *reinterpret_cast<uint2 *>(codes + s * D + lane * 8) =
-            make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+            make_uint2(codes_of(x[i].x) | codes_of(x[i].y) << 16, codes_of(x[i].z) | codes_of(x[i].w) << 16);
       }
     };
-    if ((__float_as_uint(sc) & 0x7FFFFFu) == 0) {
-      const float inv = 1.0f / sc;
-      store([&](float f) { return f * inv; });
+    const bool pow2 = (__float_as_uint(sc) & 0x7FFFFFu) == 0;
+    const float inv = 1.0f / sc;
+    if (pow2 && !BF16 && inv <= 32768.0f && inv >= 6.103515625e-05f) {
+      const __half2 f = __float2half2_rn(inv);
+      store([&](uint32_t w) {
+        const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&w), f);
+        uint16_t r;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t *>(&y)));
+        return (uint32_t)r;
+      });
+    } else if (pow2) {
+      store([&](uint32_t w) {
+        const float2 f = widen2<BF16>(w);
+        return to_e4m3x2(f.x * inv, f.y * inv);
+      });
     } else {
-      store([&](float f) { return f / sc; });
+      store([&](uint32_t w) {
+        const float2 f = widen2<BF16>(w);
+        return to_e4m3x2(f.x / sc, f.y / sc);
+      });
     }
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) x[i] = next[i];
@@ -356,12 +383,14 @@ cudaError_t launch_kv8_append(const Kv8AppendArgs &a, cudaStream_t stream) {
   const int64_t pages = ((int64_t)a.max_new - 1 + c.page_size - 1) / c.page_size + 1;
   if (pages * a.B > INT32_MAX) return cudaErrorInvalidValue;
   p.pages_per_seq = (int)pages;
-  // All items of a page in one block hide the look-up of lengths and page
-  // behind more work (37k tokens, 8 heads: 50 us against 67 with one item a
-  // block); where that would leave SMs idle, as for single tokens, fewer.
-  const int64_t items = (int64_t)c.heads * 2, blocks = (int64_t)sm_count_current() * 8;
+  // Several items in a block hide the look-up of lengths and page, and the
+  // next item's loads, behind the first one's work; more of them leave a tail
+  // in which few blocks work. 37k tokens of 8 heads with 2 / 4 / 8 / 16 items
+  // a block: 46.5 / 43.0 / 44.1 / 49.6 us; 32 single tokens with 1 / 2 / 4 / 8:
+  // 3.7 / 3.2 / 4.0 / 6.0 us.
+  const int64_t items = (int64_t)c.heads * 2;
   p.heads = c.heads;
-  p.per_block = (int)(pages * a.B >= blocks ? items : (pages * a.B * items + blocks - 1) / blocks);
+  p.per_block = pages * a.B * items >= (int64_t)sm_count_current() * 32 ? 4 : 2;
   const dim3 grid((unsigned)(pages * a.B), (unsigned)((items + p.per_block - 1) / p.per_block));
   const bool bf16 = a.dtype == VC_DTYPE_BF16;
   if (c.head_dim == 64)
