@@ -1462,27 +1462,40 @@ VCError k_native_flash(VCKernel &, const LaunchShape &, const VCKernelArg *a, in
 
 // Whether kernels of the current device can read p: its own or managed memory,
 // or pinned host memory. (What lies behind a wrong pointer would be a GPU
-// fault, so foreign memory is asked for too.)
+// fault, so foreign memory is asked for too: 0.03 us a pointer.)
 bool device_readable(const void *p) {
-  cudaPointerAttributes a;
-  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  if (a.type == cudaMemoryTypeDevice) return a.device == t_device;
-  return a.type == cudaMemoryTypeManaged || a.type == cudaMemoryTypeHost;
+  typedef CUresult (*AttributesFn)(unsigned, CUpointer_attribute *, void **, CUdeviceptr);
+  static const AttributesFn query = [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuPointerGetAttributes", &fn, 12000, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<AttributesFn>(fn);
+  }();
+  CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_IS_MANAGED,
+                                 CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+  unsigned type = 0, managed = 0;  // 0: unknown to CUDA
+  int device = -1;
+  void *to[3] = {&type, &managed, &device};
+  if (!query || query(3, what, to, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS) return false;
+  return type == CU_MEMORYTYPE_HOST || managed || (type == CU_MEMORYTYPE_DEVICE && device == t_device);
 }
-// The last step before a launch, once the arguments are known to be in order
-// (which needs no GPU): the runtime is up and every pointer is readable.
-VCError ready_to_launch(const char *k, std::initializer_list<const void *> pointers) {
-  if (!ensure_init()) return VCError::InitializationError;
-  use_current_device();
+VCError readable(const char *k, std::initializer_list<const void *> pointers) {
   for (const void *p : pointers)
     if (p && !device_readable(p)) {
       std::fprintf(stderr, "vc: kernel %s: a pointer is not memory of the current device\n", k);
       return VCError::InvalidValue;
     }
   return VCError::Success;
+}
+// The last step before a launch, once the arguments are known to be in order
+// (which needs no GPU): the runtime is up and every pointer is readable.
+VCError ready_to_launch(const char *k, std::initializer_list<const void *> pointers) {
+  if (!ensure_init()) return VCError::InitializationError;
+  use_current_device();
+  return readable(k, pointers);
 }
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -1635,9 +1648,9 @@ VCError kv8_copy_checked(const vc_kv8_cache *layers, int n_layers, const int32_t
   if (n == 0) return VCError::Success;
   VCError e = ints_checked(src, n, name);
   if (e == VCError::Success) e = ints_checked(dst, n, name);
-  for (int i = 0; i < n_layers && e == VCError::Success; ++i)
-    e = ready_to_launch(name, {layers[i].k, layers[i].v, layers[i].k_scale, layers[i].v_scale});
   if (e == VCError::Success) e = ready_to_launch(name, {src, dst});
+  for (int i = 0; i < n_layers && e == VCError::Success; ++i)
+    e = readable(name, {layers[i].k, layers[i].v, layers[i].k_scale, layers[i].v_scale});
   if (e != VCError::Success) return e;
   return run(vcb::launch_kv8_copy(layers, n_layers, src, dst, n, s), name);
 }

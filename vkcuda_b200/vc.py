@@ -190,12 +190,14 @@ def library() -> ctypes.CDLL:
 
 def _addr(x) -> Optional[int]:
     """Address of a host or device buffer (int, numpy array, ctypes object, torch tensor)."""
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or type(x) is int:
         return x
-    if hasattr(x, "data_ptr"):
+    try:  # a tensor, as the serving calls mostly get
         return x.data_ptr()
+    except AttributeError:
+        pass
+    if isinstance(x, int):
+        return int(x)
     if hasattr(x, "__array_interface__"):
         return x.__array_interface__["data"][0]
     if isinstance(x, (bytearray, memoryview)):
