@@ -172,6 +172,28 @@ def test_window_long_sampled(gpu, t):
     _window_case(gpu, t, 2, 3, 1, 4096, 4096, 128, 0, 0, rows=rows, seed=3)
 
 
+PAIR_SHAPES = [
+    # B, Hq, Hkv, Nq, Nk, window, sinks, lens: more row tiles than SMs, so that a CTA takes two, of
+    # the same rows, of adjacent ones, and none where a sequence has ended
+    (10, 16, 16, 129, 129, 0, 0, None), (6, 14, 2, 257, 257, 100, 3, None), (12, 12, 4, 150, 290, 70, 130, None),
+    (5, 32, 2, 130, 60, 16, 2, None), (40, 4, 1, 130, 130, 0, 0, [130, 1, 0, 64, 128, 129, 127, -1] * 5),
+    (9, 15, 3, 300, 300, 33, 5, [300, 0, 0, 0, 1, 257, 256, 129, 299]),
+    (8, 8, 8, 384, 384, 128, 256, [0, 0, 0, 0, 0, 0, 0, 383]),
+    (20, 8, 2, 200, 333, 90, 4, [333, 134, 133, 200] * 5), (3, 64, 64, 140, 140, 1, 0, [140, 128, 5]),
+]
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("shape", PAIR_SHAPES)
+def test_window_pairs_of_tiles(gpu, shape, d, t):
+    B, Hq, Hkv, Nq, Nk, window, sinks, lens = shape
+    assert (Nq + 127) // 128 * Hq * B > 148
+    rows = sorted({0, 1, 63, 100, 127, 128, 129, 255, 256, Nq - 2, Nq - 1} & set(range(Nq)))
+    _window_case(gpu, t, B, Hq, Hkv, Nq, Nk, d, window, sinks, lens=lens, rows=rows,
+                 tokens_first=d == 64, seed=Nq + Hq)
+
+
 def test_window_matches_flash_fwd(gpu):
     """Without a window it is the causal vc_flash_fwd."""
     B, H, N, d = 2, 3, 500, 128

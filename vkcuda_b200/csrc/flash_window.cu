@@ -111,6 +111,7 @@ struct WindowParams {
   int64_t so[3];
   bool wide;  // O's rows begin on 32 bytes
   int Hq, Hkv, Nq, Nk, window, sinks;
+  int per_cta;  // row tiles that a CTA takes at a time: 2, or 1
   float scale_log2;
 };
 
@@ -131,13 +132,14 @@ __device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Wor
   int count[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int unit = 2 * pair + w;
+    const int unit = p.per_cta * pair + w;
     const int row0 = unit / group * BQ;
     // Positions of the rows that are computed: the last one has the most keys.
     const int t_first = max(row0 + shift, 0);
     const int t_last = min(min(row0 + BQ, p.Nq) - 1 + shift, n - 1);
     kt[w] = {0, 0, 0};
-    if (unit < units && t_last >= t_first) {
+    const bool exists = w < p.per_cta && unit < units;
+    if (exists && t_last >= t_first) {
       kt[w].hi = t_last / BKV + 1;
       if (p.window > 0) {
         kt[w].lo = max(t_first - p.window + 1, 0) / BKV;
@@ -147,7 +149,7 @@ __device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Wor
     count[w] = kt[w].count();
     k.row0[w] = row0;
     k.head[w] = kvh * group + unit % group;
-    k.exists[w] = unit < units;
+    k.exists[w] = exists;
     k.count[w] = count[w];
     k.kt[w] = kt[w];
   }
@@ -739,8 +741,14 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   p.sinks = a.sinks;
   p.scale_log2 = a.scale_log2;
   const int64_t units = ((int64_t)a.Nq + BQ - 1) / BQ * (a.Hq / a.Hkv);
-  if ((units + 1) / 2 * a.B * a.Hkv > INT32_MAX / kOrderGroup) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)((units + 1) / 2), a.B * a.Hkv);
+  if (units * a.B * a.Hkv > INT32_MAX / kOrderGroup) return cudaErrorInvalidValue;
+  // One row tile a CTA while every tile can have an SM of its own: a step then
+  // takes 1.5 us instead of 1.9 (8 heads x 1024 tokens, 64 tiles: 17.7 us
+  // against 21.7; 8 x 2048, 128 tiles: 29.9 against 36.2). With more tiles than
+  // SMs two share the loads and the tensor cores' gaps (256 tiles: 37.8 us
+  // against 42.0; 1024: 86 against 117).
+  p.per_cta = units * a.B * a.Hkv <= sm_count_current() ? 1 : 2;
+  const dim3 grid((unsigned)((units + p.per_cta - 1) / p.per_cta), a.B * a.Hkv);
   if (a.d == 64)
     return bf16 ? launch_typed<64, true>(p, grid, stream) : launch_typed<64, false>(p, grid, stream);
   return bf16 ? launch_typed<128, true>(p, grid, stream) : launch_typed<128, false>(p, grid, stream);
