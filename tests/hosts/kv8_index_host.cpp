@@ -53,12 +53,17 @@ int main() {
 
   for (int64_t total : {(int64_t)1, (int64_t)2, (int64_t)7, (int64_t)147, (int64_t)148, (int64_t)149,
                         (int64_t)1000, (int64_t)4099, (int64_t)1 << 33})
-    for (int blocks : {1, 2, 3, 148, 296, 444, 592}) {
-      CHECK(split_start(total, blocks, 0) == 0 && split_start(total, blocks, blocks) == total);
-      if (total > 5000) continue;
-      for (int c = 0; c < blocks; ++c)
-        for (int64_t t = split_start(total, blocks, c); t < split_start(total, blocks, c + 1); ++t)
-          CHECK(split_owner(total, blocks, t) == c);
+    for (int most : {1, 2, 3, 148, 296, 444, 592}) {
+      const TileSplit sp(total, most);
+      CHECK(sp.blocks >= 1 && sp.blocks <= most && sp.blocks <= total);
+      CHECK(sp.start(0) == 0 && sp.start(sp.blocks) == total);
+      for (int c = 0; c < sp.blocks; ++c) {
+        const int64_t n = sp.start(c + 1) - sp.start(c);
+        CHECK(n == total / sp.blocks || n == total / sp.blocks + 1);
+        CHECK(sp.owner(sp.start(c)) == c && sp.owner(sp.start(c + 1) - 1) == c);
+        if (total < 5000)
+          for (int64_t t = sp.start(c); t < sp.start(c + 1); ++t) CHECK(sp.owner(t) == c);
+      }
     }
 
   for (int e = -140; e < 128; ++e)

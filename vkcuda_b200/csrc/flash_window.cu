@@ -230,6 +230,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   grid_dependency_wait();
+  fence_proxy_async_global();  // TMA reads what the launch before wrote
   grid_launch_dependents();
 
   // The pairs, for every warp but the scheduler: `work` waits for pair `round`

@@ -286,6 +286,43 @@ __device__ __noinline__ void join_parts(float *slots, int first, int first_slot,
   }
 }
 
+// How the parts of an item are joined: blocks first, first + 1, ... hold them,
+// part 0 in slot 1 of its block where the item starts within the block's range.
+// Up to 8 parts are joined at once; more in groups of about their root, each by
+// the block of the group that arrives last, and the groups' results by the last
+// of those.
+struct Join {
+  int first, first_slot, size, groups;
+  int from, count;  // this block's group
+  size_t lead;      // slot of its first part
+};
+// A block's part of an item [item0, item1) that other blocks have parts of.
+struct Part {
+  Join join;
+  uint16_t *out;    // the item's output rows; null: there is no part
+  int nh;
+  unsigned before;  // parts of the group that had arrived before it
+};
+__device__ __forceinline__ Join join_of(const TileSplit &split, int64_t item0, int64_t item1) {
+  Join j;
+  j.first = split.owner(item0);
+  const int parts = split.owner(item1 - 1) - j.first + 1;
+  j.first_slot = split.start(j.first) < item0 ? 1 : 0;
+  j.size = parts;
+  if (parts > 8)
+    for (j.size = 3; j.size * j.size < parts;) ++j.size;
+  j.groups = (parts + j.size - 1) / j.size;
+  j.from = ((int)blockIdx.x - j.first) / j.size * j.size;
+  j.count = min(j.size, parts - j.from);
+  j.lead = part_slot(j.first, j.first_slot, j.from);
+  return j;
+}
+__device__ __forceinline__ unsigned arrive(unsigned *counter) {
+  unsigned before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT))
 kv8_attn_kernel(const __grid_constant__ AttnParams p) {
@@ -294,8 +331,8 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int sh_scan[kWarps], sh_found[2];
-  __shared__ unsigned sh_last;
+  __shared__ Part sh_parts[2];  // of items that began, or end, in other blocks
+  __shared__ bool sh_last;
   float *const merge = reinterpret_cast<float *>(smem + S::kMerge);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, t = lane & 3;
@@ -304,40 +341,28 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
   }
+  if (tid == 0) {
+    sh_parts[0].out = sh_parts[1].out = nullptr;
+    tma_prefetch_desc(&p.k);
+    tma_prefetch_desc(&p.v);
+  }
+  __syncwarp();
   const int items = p.heads * p.groups;
 
   grid_dependency_wait();
+  fence_proxy_async_global();  // TMA reads what the launch before wrote
   grid_launch_dependents();
 
   // ---- this block's range of tiles
   auto tiles_of = [&](int b) {
     return visible_tiles(visible_keys(clamped_len(p, b), p.window, p.sinks), kTile).count;
   };
-  auto block_scan = [&](int x, int &before) {  // inclusive sum over the block, and its total
-    int s = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    __syncthreads();
-    if (lane == 31) sh_scan[warp] = s;
-    __syncthreads();
-    int total = 0, mine = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) mine += sh_scan[w];
-      total += sh_scan[w];
-    }
-    before = mine + s - x;
-    return total;
-  };
-  const int mine = tid < p.B ? tiles_of(tid) : 0;
-  int seq_tiles = mine, before;
-  for (int b = tid + kThreads; b < p.B; b += kThreads) seq_tiles += tiles_of(b);
-  const int all = block_scan(seq_tiles, before);
-  const int64_t total = (int64_t)all * items;
-  const int blocks = (int)(total < gridDim.x ? total : gridDim.x);
+  // Every warp finds it for itself, 32 sequences at a time.
+  const int n0 = lane < p.B ? tiles_of(lane) : 0;
+  int seq_tiles = n0;
+  for (int b = lane + 32; b < p.B; b += 32) seq_tiles += tiles_of(b);
+  const int64_t total = (int64_t)__reduce_add_sync(0xffffffffu, seq_tiles) * items;
+  const TileSplit split(total > 0 ? total : 1, gridDim.x);
 
   // Sequences without a token: zero rows.
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
@@ -347,33 +372,32 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     uint4 *row = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.O) + b * p.o_stride);
     for (int i = tid; i < p.heads * p.group * D / 8; i += kThreads) row[i] = make_uint4(0, 0, 0, 0);
   }
-  if ((int)blockIdx.x >= blocks) return;
-  const int64_t t0 = split_start(total, blocks, blockIdx.x);
-  const int64_t t1 = split_start(total, blocks, blockIdx.x + 1);
-  if (tid == 0) sh_found[0] = -1;
-  __syncthreads();
-  auto found = [&](int b, int n, int64_t first) {
-    if (t0 < first || t0 >= first + (int64_t)n * items) return;
-    sh_found[0] = b;
-    sh_found[1] = (int)(t0 - first);
-  };
-  if (p.B <= kThreads) {
-    found(tid, mine, (int64_t)before * items);
-  } else {
-    int64_t base = 0;  // tiles before the chunk of sequences, times items
-    for (int b0 = 0; b0 < p.B && base <= t0; b0 += kThreads) {
-      const int n = b0 + tid < p.B ? tiles_of(b0 + tid) : 0;
-      const int chunk = block_scan(n, before);
-      found(b0 + tid, n, base + (int64_t)before * items);
-      base += (int64_t)chunk * items;
-    }
-  }
-  __syncthreads();
-  if (sh_found[0] < 0) return;
+  if (total == 0 || (int)blockIdx.x >= split.blocks) return;
+  const int64_t t0 = split.start(blockIdx.x), t1 = split.start(blockIdx.x + 1);
   Cursor cur;
-  set_sequence(cur, p, sh_found[0]);
-  cur.item = sh_found[1] / cur.tiles.count;
-  cur.tile = sh_found[1] % cur.tiles.count;
+  cur.b = -1;
+  int64_t base = 0;  // tiles before these 32 sequences
+  for (int b0 = 0; b0 < p.B && cur.b < 0; b0 += 32) {
+    const int n = b0 == 0 ? n0 : b0 + lane < p.B ? tiles_of(b0 + lane) : 0;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const int64_t begin = base + (int64_t)(upto - n) * items;
+    const unsigned hit = __ballot_sync(0xffffffffu, t0 >= begin && t0 < begin + (int64_t)n * items);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int off = __shfl_sync(0xffffffffu, (int)(t0 - begin), src);
+      set_sequence(cur, p, b0 + src);
+      const int count = __shfl_sync(0xffffffffu, n, src);
+      cur.item = off / count;
+      cur.tile = off - cur.item * count;
+    }
+    base += (int64_t)__shfl_sync(0xffffffffu, upto, 31) * items;
+  }
+  if (cur.b < 0) return;  // (lengths that change underneath)
 
   // ---- the warp's ring
   uint8_t *const ring = smem + warp * kStages * S::kStage;
@@ -770,44 +794,42 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
         }
       }
     }
-    if (!whole) {
-      // ---- blocks first .. last hold parts of this item
-      const int first = split_owner(total, blocks, item0), last = split_owner(total, blocks, item1 - 1);
-      const int parts = last - first + 1;
-      // Up to 8 parts are joined at once; more in groups of about their root.
-      int size = parts;
-      if (parts > 8)
-        for (size = 3; size * size < parts;) ++size;
-      const int groups = (parts + size - 1) / size;
-      // A part's slot: 1 where the item starts within the block's range.
-      const int first_slot = split_start(total, blocks, first) < item0 ? 1 : 0;
-      // Counts this block in; true for the one that completes `of`. The block's
-      // stores are behind the barrier, and the one acquire-release addition
-      // orders them before, and the others' stores after, for all of it.
-      auto arrive = [&](unsigned *counter, int of) {
-        __syncthreads();
-        if (tid == 0) {
-          unsigned before2;
-          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before2) : "l"(counter) : "memory");
-          sh_last = before2 + 1 == (unsigned)of;
-          if (sh_last) *counter = 0;  // ready for the next call
-        }
-        __syncthreads();
-        return sh_last != 0;
-      };
-      const int part = (int)blockIdx.x - first, g = part / size;
-      const int ga = g * size, gb = min(ga + size, parts);
-      const size_t lead = part_slot(first, first_slot, ga);
-      if (arrive(&p.counters[lead >> 1].group[lead & 1], gb - ga)) {
-        join_parts<D, NT, BF16>(p.slots, first, first_slot, ga, gb - ga, 1, groups == 1 ? out : nullptr, nh);
-        if (groups > 1 && arrive(&p.counters[first].item, groups))
-          join_parts<D, NT, BF16>(p.slots, first, first_slot, 0, groups, size, out, nh);
+    // A part is counted in at once, but its join, where it falls to this block,
+    // waits for the block's own work, which may be what others wait for.
+    if (!whole && warp == 0) {
+      __syncwarp();  // the warp's stores come before the arrival
+      if (lane == 0) {
+        Part &part = sh_parts[at_tile + n < t1 ? 0 : 1];
+        part.join = join_of(split, item0, item1);
+        part.out = out;
+        part.nh = nh;
+        part.before = arrive(&p.counters[part.join.lead >> 1].group[part.join.lead & 1]);
       }
     }
     __syncthreads();  // the merge buffer is free again
     at_tile += n;
     cur.tile += n;
     if (at_tile < t1) next_item(cur, p);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const Part part = sh_parts[i];
+    const Join &j = part.join;
+    if (!part.out || part.before + 1 != (unsigned)j.count) continue;  // another block is the last
+    if (tid == 0) p.counters[j.lead >> 1].group[j.lead & 1] = 0;      // ready for the next call
+    __threadfence();
+    join_parts<D, NT, BF16>(p.slots, j.first, j.first_slot, j.from, j.count, 1,
+                            j.groups == 1 ? part.out : nullptr, part.nh);
+    if (j.groups == 1) continue;
+    __syncthreads();
+    if (tid == 0) {
+      sh_last = arrive(&p.counters[j.first].item) + 1 == (unsigned)j.groups;
+      if (sh_last) p.counters[j.first].item = 0;
+    }
+    __syncthreads();
+    if (sh_last)
+      join_parts<D, NT, BF16>(p.slots, j.first, j.first_slot, 0, j.groups, j.size, part.out, part.nh);
   }
   // Only a wait that ran out leaves copies behind: they get time to land.
   for (int i = 0; !ok && i < kStages; ++i) {

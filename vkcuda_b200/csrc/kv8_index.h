@@ -50,12 +50,23 @@ VCB_HD int tile_key(const VisibleTiles &t, int i, int tile) {
   return (i < t.head ? i : t.first + (i - t.head)) * tile;
 }
 
-// Split of `total` tiles over `blocks` blocks: block c takes [start(c), start(c + 1)).
-VCB_HD int64_t split_start(int64_t total, int blocks, int c) { return total * c / blocks; }
-// The block that takes tile t: the largest c with start(c) <= t.
-VCB_HD int split_owner(int64_t total, int blocks, int64_t t) {
-  return (int)(((t + 1) * blocks + total - 1) / total - 1);
-}
+// Split of `total` > 0 tiles over at most `most` blocks, as even as it gets:
+// block c takes [start(c), start(c + 1)), the first `more` blocks one tile more.
+struct TileSplit {
+  int64_t each;
+  int blocks, more;
+  VCB_HD TileSplit(int64_t total, int most) {
+    blocks = total < most ? (int)total : most;
+    each = total / blocks;
+    more = (int)(total - each * blocks);
+  }
+  VCB_HD int64_t start(int c) const { return each * c + (c < more ? c : more); }
+  // The block that takes tile t.
+  VCB_HD int owner(int64_t t) const {
+    const int64_t head = (each + 1) * more;
+    return t < head ? (int)(t / (each + 1)) : more + (int)((t - head) / each);
+  }
+};
 
 // Scale of a block whose largest finite magnitude is `amax`: 2^e, e the
 // smallest exponent with amax <= 448 * 2^e (448: the largest e4m3 value,

@@ -287,6 +287,7 @@ __global__ void __launch_bounds__(64) kv8_copy_kernel(const __grid_constant__ Co
   }
   __syncthreads();
   grid_dependency_wait();
+  fence_proxy_async_global();  // the bulk copies read what the launch before wrote
   grid_launch_dependents();
   const int64_t per_pair = (int64_t)p.layers * 2 * p.chunks;
   if (threadIdx.x >= 32) {
