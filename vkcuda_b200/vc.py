@@ -586,9 +586,13 @@ def flash_fwd(Q, K, V, O, BH: int, N: int, d: int, scale_log2: float, causal: bo
 
 
 # ------------------------------------------------------------ serving entries
+_ERRORS = tuple(VCError)        # by value: their construction is a tenth of a short call
+_Strides = ctypes.c_int64 * 3
+
+
 def _strides(s):
     """Three element strides (batch, head, token), or None for a dense [B][H][N][d]."""
-    return None if s is None else (ctypes.c_int64 * 3)(*s)
+    return None if s is None else _Strides(*s)
 
 
 def flash_window_fwd(Q, K, V, O, B: int, Hq: int, Hkv: int, Nq: int, Nk: int, d: int,
@@ -597,10 +601,10 @@ def flash_window_fwd(Q, K, V, O, B: int, Hq: int, Hkv: int, Nq: int, Nk: int, d:
                      stream=None) -> VCError:
     """Causal attention of prompts through a sliding window with sinks, K/V heads
     shared by groups of query heads (vc_flash_window_fwd)."""
-    return VCError(library().vc_flash_window_fwd(
+    return _ERRORS[library().vc_flash_window_fwd(
         _addr(Q), _addr(K), _addr(V), _addr(O), B, Hq, Hkv, Nq, Nk, d, _strides(q_strides),
         _strides(k_strides), _strides(v_strides), _strides(o_strides), _addr(lens), window, sinks,
-        float(scale_log2), int(dtype), _stream(stream)))
+        float(scale_log2), int(dtype), _stream(stream))]
 
 
 class Kv8Cache(ctypes.Structure):
@@ -629,10 +633,10 @@ def kv8_append(cache: Kv8Cache, K, V, tokens: int, table, table_width: int, star
                v_stride: int = 0, stream=None) -> VCError:
     """Quantise new K/V tokens into their sequences' pages (vc_kv8_append); strides 0: dense."""
     row = cache.heads * cache.head_dim
-    return VCError(library().vc_kv8_append(
+    return _ERRORS[library().vc_kv8_append(
         ctypes.byref(cache), _addr(K), _addr(V), k_stride or row, v_stride or row, tokens,
         _addr(table), table_width, _addr(start), _addr(cu), B, max_new, _addr(lens_out), int(dtype),
-        _stream(stream)))
+        _stream(stream))]
 
 
 def kv8_attn_workspace(cache: Kv8Cache, B: int, Hq: int) -> Tuple[VCError, int]:
@@ -647,16 +651,16 @@ def kv8_attn(cache: Kv8Cache, Q, O, table, table_width: int, lens, B: int, Hq: i
              sinks: int = 0, q_stride: int = 0, o_stride: int = 0, stream=None) -> VCError:
     """Attention of one token for each sequence over the cache (vc_kv8_attn); strides 0: dense."""
     row = Hq * cache.head_dim
-    return VCError(library().vc_kv8_attn(
+    return _ERRORS[library().vc_kv8_attn(
         ctypes.byref(cache), _addr(Q), q_stride or row, _addr(O), o_stride or row, _addr(table),
         table_width, _addr(lens), B, Hq, window, sinks, float(scale_log2), int(dtype),
-        _addr(workspace), workspace_bytes, _stream(stream)))
+        _addr(workspace), workspace_bytes, _stream(stream))]
 
 
 def kv8_copy_pages(layers, src, dst, n: int, stream=None) -> VCError:
     """Copy pages src[i] -> dst[i] in every layer (kv8_layers), codes and scales."""
-    return VCError(library().vc_kv8_copy_pages(layers, len(layers), _addr(src), _addr(dst), n,
-                                               _stream(stream)))
+    return _ERRORS[library().vc_kv8_copy_pages(layers, len(layers), _addr(src), _addr(dst), n,
+                                               _stream(stream))]
 
 
 def kv8_pool_create(num_pages: int, page_size: int) -> Tuple[VCError, int]:
