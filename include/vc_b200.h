@@ -325,7 +325,9 @@ int vc_kv8_append(const vc_kv8_cache *cache, const void *K, const void *V, int64
  * are several rows with the same pages and growing lens.
  * workspace: vc_kv8_attn_workspace bytes, 256-byte aligned, zero before its
  * first call and left ready for the next, of whatever shape; calls that may
- * overlap (two streams, two graphs) need one each. */
+ * overlap (two streams, two graphs) need one each, and after a kernel error 1
+ * (a wait that ran out) it is zeroed again. The scores have to be finite in
+ * fp32; batch and table sizes with 2^31 or more tiles of 128 keys are refused. */
 int vc_kv8_attn_workspace(const vc_kv8_cache *cache, int B, int Hq, size_t *bytes);
 int vc_kv8_attn(const vc_kv8_cache *cache, const void *Q, int64_t q_stride, void *O,
                 int64_t o_stride, const int32_t *table, int table_width, const int32_t *lens,
