@@ -172,6 +172,12 @@ def test_window_long_sampled(gpu, t):
     _window_case(gpu, t, 2, 3, 1, 4096, 4096, 128, 0, 0, rows=rows, seed=3)
 
 
+def test_window_late_rows_of_a_long_sequence(gpu):
+    """The last rows of 300000 tokens, through a window and in full."""
+    _window_case(gpu, torch.float16, 1, 2, 1, 4, 300000, 64, 1000, 130, seed=5)
+    _window_case(gpu, torch.bfloat16, 1, 1, 1, 2, 200001, 128, 0, 0, seed=6)
+
+
 PAIR_SHAPES = [
     # B, Hq, Hkv, Nq, Nk, window, sinks, lens: more row tiles than SMs, so that a CTA takes two, of
     # the same rows, of adjacent ones, and none where a sequence has ended
@@ -510,6 +516,84 @@ def test_attn_strided_rows(gpu):
     _done(gpu)
     assert torch.equal(out[:, :Hq * d].reshape(3, Hq, d), dense)
     assert (out[:, Hq * d:] == 7.0).all()
+
+
+@pytest.mark.parametrize("B", [33, 300, 1500])
+def test_attn_many_short_sequences(gpu, B):
+    """More sequences than a warp has lanes, empty ones among them, in any order."""
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, 40, B).tolist()
+    lens[0], lens[B // 2], lens[-1] = 0, 700, 0
+    c, table = _fill(gpu, lens, 2, 16, 64, rng)
+    _attn_case(gpu, c, table, lens, 6, torch.float16, 0, 0)
+    _attn_case(gpu, c, table, lens, 6, torch.bfloat16, 17, 2)
+    zeros = [0] * B
+    q, o = _attn_case(gpu, c, table, zeros, 6, torch.float16, 0, 0, check=False)
+    assert (o == 0).all()
+
+
+def test_attn_very_long(gpu):
+    """300000 tokens of one sequence; offsets, splits and joins of the longest kind."""
+    rng = np.random.default_rng(31)
+    lens = [300001]
+    c, table = _fill(gpu, lens, 1, 128, 64, rng)
+    _attn_case(gpu, c, table, lens, 2, torch.float16, 0, 0)
+    _attn_case(gpu, c, table, lens, 16, torch.bfloat16, 200000, 4)
+
+
+def test_attn_nan_query_stays_in_its_row(gpu):
+    rng = np.random.default_rng(32)
+    lens = [5000, 40]
+    c, table = _fill(gpu, lens, 1, 32, 128, rng)
+    q, clean = _attn_case(gpu, c, table, lens, 8, torch.float16, 0, 0)
+    q2 = q.clone()
+    q2[0, 3, 7] = float("nan")
+    o = torch.empty_like(q2)
+    err, n = gpu.kv8_attn_workspace(c.handle, 2, 8)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    assert gpu.kv8_attn(c.handle, q2, o, _ints(table), table.shape[1], _ints(lens), 2, 8,
+                        LOG2E / math.sqrt(128), gpu.Dtype.F16, ws, n) == 0
+    _done(gpu)
+    assert torch.isnan(o[0, 3]).all()
+    keep = torch.ones(2, 8, dtype=torch.bool)
+    keep[0, 3] = False
+    # The running maximum may move at other keys: fp32 roundings, then one of the output.
+    assert (o[keep].double() - clean[keep].double()).abs().max() <= 2.0 ** -10 * clean.abs().max()
+
+
+def test_layers_in_one_allocation(gpu):
+    """Append and attention on two layers whose pages alternate in memory, K and V and the scales
+    of both in one buffer each."""
+    H, P, d, pages, Hq = 2, 32, 64, 9, 6
+    one = H * P * d
+    codes = torch.full((pages, 2, 2, one + 64), 0x7F, dtype=torch.uint8, device="cuda")
+    scales = torch.full((pages, 2, 2, H + 3), 5.0, device="cuda")
+    want = [codes.clone(), scales.clone()]
+    caches = [gpu.kv8_cache(codes[0, i, 0], codes[0, i, 1], scales[0, i, 0], scales[0, i, 1], pages, H, P, d,
+                            page_stride=4 * (one + 64), scale_stride=4 * (H + 3)) for i in range(2)]
+    rng = np.random.default_rng(3)
+    lens = [70, 33]
+    table = _table(lens, P, pages, rng)
+    ws = torch.zeros(gpu.kv8_attn_workspace(caches[0], 2, Hq)[1], dtype=torch.uint8, device="cuda")
+    for i in range(2):
+        x = [torch.randn(103, H, d, device="cuda").half() for _ in range(2)]
+        q, o = torch.randn(2, Hq, d, device="cuda").half(), torch.empty(2, Hq, d, device="cuda").half()
+        assert gpu.kv8_append(caches[i], x[0], x[1], 103, _ints(table), 3, _ints([0, 0]), 2, 70, gpu.Dtype.F16,
+                              cu=_ints([0, 70, 103])) == 0
+        assert gpu.kv8_attn(caches[i], q, o, _ints(table), 3, _ints(lens), 2, Hq, 0.18, gpu.Dtype.F16, ws,
+                            ws.numel()) == 0
+        _done(gpu)
+        host = []
+        for kv in range(2):
+            ck = np.full((pages, H, P, d), 0x7F, np.uint8)
+            sk = np.full((pages, H), 5.0, np.float32)
+            plain.append(ck, sk, _f64(x[kv]), table, [0, 0], lens, P)
+            want[0][:, i, kv, :one] = torch.from_numpy(ck.reshape(pages, one)).cuda()
+            want[1][:, i, kv, :H] = torch.from_numpy(sk).cuda()
+            host += [ck, sk]
+        assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+        exp = plain.cache_attn(_f64(q), *host, table, lens, 0, 0, 0.18, P)
+        assert np.abs(_f64(o) - exp).max() <= 2.0 ** -11 * 3 * 6 + 1e-4
 
 
 def test_attn_reports_bad_pages_and_lengths(gpu):
