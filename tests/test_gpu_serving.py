@@ -281,6 +281,25 @@ def test_append_exact(gpu, P, d, t):
             assert np.array_equal(g, w), (name, size, np.argwhere(g != w)[:4])
 
 
+def test_append_nothing(gpu):
+    """A step in which no sequence has new tokens: empty tensors, the lengths as they were."""
+    rng = np.random.default_rng(5)
+    c, table = _fill(gpu, [30, 7], 2, 16, 64, rng)
+    before = c.host()
+    for t, cu in ((torch.half, _ints([0, 0, 0])), (torch.bfloat16, None)):
+        none = torch.empty(0, 2, 64, device="cuda", dtype=t)
+        assert none.data_ptr() == 0
+        lens = _ints([-1, -1])
+        assert gpu.kv8_append(c.handle, none, none, 0, _ints(table), table.shape[1], _ints([30, 7]), 2,
+                              4 if cu is not None else 0, _dt(gpu, t), cu=cu, lens_out=lens) == 0
+        _done(gpu)
+        assert lens.tolist() == [30, 7]
+    for g, w in zip(c.host(), before):
+        assert np.array_equal(g, w)
+    assert gpu.kv8_append(c.handle, None, None, 1, _ints(table), table.shape[1], _ints([30, 7]), 1, 1,
+                          gpu.Dtype.F16) == gpu.VCError.InvalidValue
+
+
 def test_append_step_strided(gpu):
     """One token each, out of a fused projection, without offsets; extreme magnitudes keep their
     scales within range."""

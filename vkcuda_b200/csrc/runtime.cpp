@@ -1572,9 +1572,10 @@ VCError kv8_cache_checked(const vc_kv8_cache &c, const char *name) {
 }
 // Rows of `width` 16-bit elements, `stride` apart.
 VCError rows_checked(const void *p, int64_t rows, int64_t width, int64_t stride, const char *name) {
-  if (!p || !aligned(p, 16) || stride < width || stride % 8 || stride > (int64_t)1 << 38)
+  if (!aligned(p, 16) || stride < width || stride % 8 || stride > (int64_t)1 << 38)
     return VCError::InvalidValue;
-  if (rows <= 0) return VCError::Success;
+  if (rows <= 0) return VCError::Success;  // an empty tensor may be null
+  if (!p) return VCError::InvalidValue;
   return (size_t)((rows - 1) * stride + width) * 2 > bytes_available(p) ? too_small(name)
                                                                         : VCError::Success;
 }
