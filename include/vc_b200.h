@@ -256,9 +256,10 @@ int vc_flash_fwd(const void *Q, const void *K, const void *V, void *O, int BH,
                  void *stream);
 
 /* ---- Serving entries. Beside the usual errors they refuse, with
- * VC_INVALID_VALUE and before any launch, a pointer that this device cannot
- * read (host memory, another device's). With `stream` NULL they join a graph
- * that is being recorded (vc_graph_begin_record), as vc_launch_kernel does.
+ * VC_INVALID_VALUE and before any launch, a pointer that is not this device's
+ * own memory (host, pinned or managed memory, another device's). With `stream`
+ * NULL they join a graph that is being recorded (vc_graph_begin_record), as
+ * vc_launch_kernel does.
  * What lies in device memory (lengths, offsets, page numbers) is checked by
  * the kernels: what is out of range is left out and vc_kernel_error reports
  * it (4, out of bounds). */

@@ -729,6 +729,31 @@ def test_host_pointers_are_refused(gpu):
     _done(gpu)
 
 
+def test_pinned_and_managed_memory_are_refused(gpu):
+    rng = np.random.default_rng(2)
+    c, table = _fill(gpu, [30], 1, 16, 64, rng)
+    q = torch.zeros(1, 4, 64, device="cuda").half()
+    ws = torch.zeros(1 << 24, dtype=torch.uint8, device="cuda")
+    pinned = torch.zeros(1 << 14, dtype=torch.uint8).pin_memory()
+    err, managed = gpu.vcMallocManaged(1 << 14)
+    assert err == 0
+    try:
+        for other in (pinned, managed):
+            tail = (_ints(table), table.shape[1], _ints([30]), 1, 4, 0.1, gpu.Dtype.F16, ws, ws.numel())
+            assert gpu.kv8_attn(c.handle, other, q, *tail) == gpu.VCError.InvalidValue
+            bad = gpu.kv8_cache(other, c.v, c.ks, c.vs, 2, 1, 16, 64)
+            assert gpu.kv8_attn(bad, q, q, *tail) == gpu.VCError.InvalidValue
+            assert gpu.kv8_append(c.handle, q, q, 1, other, 1, _ints([0]), 1, 1, gpu.Dtype.F16) \
+                == gpu.VCError.InvalidValue
+            assert gpu.kv8_copy_pages(gpu.kv8_layers([bad]), _ints([0]), _ints([1]), 1) \
+                == gpu.VCError.InvalidValue
+            assert gpu.flash_window_fwd(q, other, q, q, 1, 4, 4, 1, 1, 64, 0.1, gpu.Dtype.F16) \
+                == gpu.VCError.InvalidValue
+    finally:
+        assert gpu.vcFree(managed) == 0
+    _done(gpu)
+
+
 def test_buffers_too_small_are_refused(gpu, dev):
     small = dev.alloc(4096)
     assert gpu.flash_window_fwd(small.ptr, small.ptr, small.ptr, small.ptr, 1, 4, 4, 64, 64, 64, 0.1,

@@ -1460,10 +1460,10 @@ VCError k_native_flash(VCKernel &, const LaunchShape &, const VCKernelArg *a, in
 
 // ---- serving entries: prompt attention through a window, 8-bit paged cache
 
-// Whether kernels of the current device can read p: its own or managed memory,
-// or pinned host memory. (What lies behind a wrong pointer would be a GPU
-// fault, so foreign memory is asked for too: 0.03 us a pointer.)
-bool device_readable(const void *p) {
+// Whether p is the current device's own memory. (What lies behind a wrong
+// pointer would be a GPU fault: 0.03 us a pointer. Managed and pinned memory are
+// refused as well: the bulk copies are for memory that stays on the device.)
+bool device_memory(const void *p) {
   typedef CUresult (*AttributesFn)(unsigned, CUpointer_attribute *, void **, CUdeviceptr);
   static const AttributesFn query = [] {
     void *fn = nullptr;
@@ -1480,22 +1480,22 @@ bool device_readable(const void *p) {
   int device = -1;
   void *to[3] = {&type, &managed, &device};
   if (!query || query(3, what, to, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS) return false;
-  return type == CU_MEMORYTYPE_HOST || managed || (type == CU_MEMORYTYPE_DEVICE && device == t_device);
+  return type == CU_MEMORYTYPE_DEVICE && !managed && device == t_device;
 }
-VCError readable(const char *k, std::initializer_list<const void *> pointers) {
+VCError on_device(const char *k, std::initializer_list<const void *> pointers) {
   for (const void *p : pointers)
-    if (p && !device_readable(p)) {
+    if (p && !device_memory(p)) {
       std::fprintf(stderr, "vc: kernel %s: a pointer is not memory of the current device\n", k);
       return VCError::InvalidValue;
     }
   return VCError::Success;
 }
 // The last step before a launch, once the arguments are known to be in order
-// (which needs no GPU): the runtime is up and every pointer is readable.
+// (which needs no GPU): the runtime is up and every pointer is this device's.
 VCError ready_to_launch(const char *k, std::initializer_list<const void *> pointers) {
   if (!ensure_init()) return VCError::InitializationError;
   use_current_device();
-  return readable(k, pointers);
+  return on_device(k, pointers);
 }
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -1651,7 +1651,7 @@ VCError kv8_copy_checked(const vc_kv8_cache *layers, int n_layers, const int32_t
   if (e == VCError::Success) e = ints_checked(dst, n, name);
   if (e == VCError::Success) e = ready_to_launch(name, {src, dst});
   for (int i = 0; i < n_layers && e == VCError::Success; ++i)
-    e = readable(name, {layers[i].k, layers[i].v, layers[i].k_scale, layers[i].v_scale});
+    e = on_device(name, {layers[i].k, layers[i].v, layers[i].k_scale, layers[i].v_scale});
   if (e != VCError::Success) return e;
   return run(vcb::launch_kv8_copy(layers, n_layers, src, dst, n, s), name);
 }
