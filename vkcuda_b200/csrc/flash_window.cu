@@ -9,9 +9,9 @@
 //
 // Bound: the tensor cores, 4 d operations per visible (row, key) pair.
 // Measured (bf16, 32 heads over 8 K/V heads of 128): 8192 tokens through a
-// window of 2048 251 us, 960 TFLOP/s of visible work; the last 2048 of 6144
-// through 4096 269 us, 1027 TFLOP/s (0.62 of the dense peak). A step of 128 keys
-// for both row tiles takes ~3700 cycles, of which the MMAs are 2048; the issuing
+// window of 2048 246 us, 980 TFLOP/s of visible work; the last 2048 of 6144
+// through 4096 268 us, 1030 TFLOP/s (0.62 of the dense peak). A step of 128 keys
+// for both row tiles takes ~3600 cycles, of which the MMAs are 2048; the issuing
 // warp spends ~2500 (75 to 80 cycles an MMA) and waits ~900 for P.
 //
 // The pipeline is the one of the plain forward (flash_fwd_tcgen05.cu): one CTA
@@ -19,7 +19,7 @@
 // of two stages of (V(u - 1), K(u)), one thread that issues the MMAs
 //   S_w = Q_w K^T (shared memory), O_w += P_w V (P_w in TMEM),
 // so that the softmax of one tile runs under the MMAs of the other, P handed
-// over in two halves, O rescaled when the maximum grows by more than 2^8.
+// over in two parts, O rescaled when the maximum grows by more than 2^8.
 //
 // The CTAs are persistent: each takes its next pair of row tiles from the
 // grid's queue (cluster launch control), and the steps of one pair follow on
@@ -61,8 +61,10 @@ constexpr int kWgThreads = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows x 64 16-bit elements
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
-constexpr int kHandoffs = 2;               // parts in which P reaches the MMAs
-constexpr int kChunksPerHandoff = (BKV / 32) / kHandoffs;
+// P reaches the MMAs in two parts: 96 keys, whose products run under the
+// exponentials of the last 32, and those, whose products are all that the next
+// scores wait for (64 + 64 took 2 to 3 % longer, four parts of 32 7 %).
+constexpr int kFirstKeys = 96;
 // K/V slices per ordering group (heaviest CTAs of every slice of a group first).
 constexpr int kOrderGroup = 8;
 
@@ -97,7 +99,7 @@ struct __align__(16) WindowBarriers {
   uint64_t kv_empty[kStages];
   uint64_t v_dirty, v_clean;  // the last V tile of a padded sequence is there; is zeroed
   uint64_t s_full[2];
-  uint64_t p_full[2][kHandoffs];
+  uint64_t p_full[2][2];
   uint64_t o_full[2], o_empty[2];
   uint32_t tmem_base;
 };
@@ -223,7 +225,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     mbar_init(&bars->v_clean, 1);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&bars->s_full[w], 1);
-      for (int h = 0; h < kHandoffs; ++h)
+      for (int h = 0; h < 2; ++h)
         mbar_init(&bars->p_full[w][h], kWgThreads / 32);  // one per warp
       mbar_init(&bars->o_full[w], 1);
       mbar_init(&bars->o_empty[w], kWgThreads / 32);
@@ -287,12 +289,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         const int key0 = tile * BKV;
         // The whole S row in registers with one wait.
         uint32_t s[BKV / 32][32];
-        if constexpr (BF16) {
-#pragma unroll
-          for (int c = 0; c < BKV / 32; ++c) tmem_ld32(s_col + c * 32, s[c]);
-        } else {
-          tmem_ld128(s_col, *reinterpret_cast<uint32_t(*)[128]>(&s[0][0]));
-        }
+        tmem_ld128(s_col, *reinterpret_cast<uint32_t(*)[128]>(&s[0][0]));
         tmem_ld_wait();
         // Keys key0 + x of this row: hidden from x = end on, and below `begin`
         // where they are no sinks (x >= keep).
@@ -334,7 +331,6 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         }
         const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
         const bool rescale_o = rescale && !first;  // warp-uniform
-        int handed = 0;                           // parts of P handed over
         // P = exp2(scale_log2 * s - m) -> 16-bit pairs over S columns.
         float lsp[4] = {0.f, 0.f, 0.f, 0.f};
         const float neg_m = -m_use, scale = p.scale_log2;
@@ -373,16 +369,11 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
               tmem_st32(o_col + oc * 32, o);
             }
           }
-          // Hand over every part whose P is complete (with an O rescale
-          // pending, not before it is done).
-          if ((c + 1) % kChunksPerHandoff == 0 && (!rescale_o || c >= 1)) {
+          if ((c + 1) * 32 >= kFirstKeys) {  // a part is complete
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            const int upto = c / kChunksPerHandoff;
-            if (lane == 0)
-              for (int h = handed; h <= upto; ++h) mbar_arrive(&bars->p_full[w][h]);
-            handed = upto + 1;
+            if (lane == 0) mbar_arrive(&bars->p_full[w][(c + 1) * 32 > kFirstKeys]);
           }
         }
         l_run += (lsp[0] + lsp[1]) + (lsp[2] + lsp[3]);
@@ -629,16 +620,14 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
           for (int w = 0; w < 2; ++w) {
             if (pv[w]) {
               const uint32_t o_tmem = tm + 256 + w * 128, p_tmem = tm + w * 128;
-              constexpr int kSteps = (BKV / 16) / kHandoffs;  // K = 16 MMAs per part
 #pragma unroll
-              for (int h = 0; h < kHandoffs; ++h) {
+              for (int h = 0; h < 2; ++h) {
                 wait(&bars->p_full[w][h], n_p[w] & 1);
                 // The last pair's O has been read.
                 if (h == 0 && !begun[w]) wait(&bars->o_empty[w], (n_o[w] & 1) ^ 1);
                 tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < kSteps; ++kk) {
-                  const int ks = h * kSteps + kk;
+                for (int ks = h ? kFirstKeys / 16 : 0; ks < (h ? BKV : kFirstKeys) / 16; ++ks) {  // K = 16 MMAs
                   mma_f16_ts_lohi_warp(o_tmem, p_tmem + ks * 8, v_lo + ks * ((16 * 128) >> 4), dv_hi,
                                        idesc_o, (begun[w] || ks > 0) ? 1u : 0u);
                 }
@@ -755,8 +744,8 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   // One row tile a CTA while every tile can have an SM of its own: a step then
   // takes 1.5 us instead of 1.9 (8 heads x 1024 tokens, 64 tiles: 17.7 us
   // against 21.7; 8 x 2048, 128 tiles: 29.9 against 36.2). With more tiles than
-  // SMs two share the loads and the tensor cores' gaps (256 tiles: 37.8 us
-  // against 42.0; 1024: 86 against 117).
+  // SMs two share the loads and the tensor cores' gaps (256 tiles: 36.0 us
+  // against 42.0; 1024: 85 against 117).
   p.per_cta = units * a.B * a.Hkv <= sm_count_current() ? 1 : 2;
   const dim3 grid((unsigned)((units + p.per_cta - 1) / p.per_cta), a.B * a.Hkv);
   if (a.d == 64)
