@@ -108,11 +108,13 @@ template <int HD>
 struct WindowSmem {
   static constexpr uint32_t kTile = (HD / 64) * kBoxBytes;  // one Q, K or V tile
   static constexpr uint32_t kRing = 2 * kTile;              // behind the two Q tiles
-  static constexpr uint32_t kBars = kRing + kStages * 2 * kTile;
+  static constexpr uint32_t kOut = kRing + kStages * 2 * kTile;  // 4 KiB a softmax warp
+  static constexpr uint32_t kBars = kOut + 8 * 4096;
   static constexpr size_t kUsed = 1024 + kBars + sizeof(WindowBarriers);
   // At least 120 KiB so that a second CTA never shares the SM: each CTA
   // allocates all 512 TMEM columns.
   static constexpr size_t kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
+  static_assert(kBytes <= 227 * 1024, "shared memory of a block");
 };
 
 struct WindowParams {
@@ -120,7 +122,6 @@ struct WindowParams {
   const int32_t *lens;
   uint16_t *O;
   int64_t so[3];
-  bool wide;  // O's rows begin on 32 bytes
   int Hq, Hkv, Nq, Nk, window, sinks;
   int per_cta;  // row tiles that a CTA takes at a time: 2, or 1
   float scale_log2;
@@ -177,13 +178,6 @@ __device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Wor
   // V's rows behind the end of a padded sequence are zeroed in its last tile:
   // their weights are 0, but 0 times what they hold may not be.
   k.clean = n < p.Nk && hi > 0 && hi * BKV > n;
-}
-
-// 32 bytes, a whole sector, to a 32-byte aligned address.
-__device__ __forceinline__ void st_global_32(void *p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
 }
 
 template <bool BF16>
@@ -267,6 +261,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t s_col = tmem + lane_off + w * 128;
     const uint32_t o_col = tmem + lane_off + 256 + w * 128;
+    const uint32_t stage = smem_u32(smem + L::kOut) + warp * 4096;
     int n_s = 0, n_o = 0;  // S tiles and O tiles so far
     bool ok = true;
     for (; wait_work(round) && bars->work[round & 1].valid; done()) {
@@ -380,13 +375,14 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         first = false;
         if (!ok) break;
       }
-      // O / l -> 16-bit. Rows of the sequence (t < n); a row without a key is
-      // zero.
-      const bool my_row = row0 + row < p.Nq && (!p.lens || t < n);
-      uint16_t *out = p.O + k.b * p.so[0] + head * p.so[1] + (int64_t)(row0 + row) * p.so[2];
+      // O / l -> 16-bit. The warp's rows of the sequence (t < n); a row without a
+      // key is zero.
+      const int rows_of_warp = min(p.Nq - row0, n - t_first) - quad * 32;
+      uint16_t *out = p.O + k.b * p.so[0] + head * p.so[1] + (int64_t)(row0 + quad * 32) * p.so[2];
       if (count == 0) {
-        if (k.exists[w] && my_row && t < 0)
-          for (int c = 0; c < HD / 8; ++c) reinterpret_cast<uint4 *>(out)[c] = make_uint4(0, 0, 0, 0);
+        if (k.exists[w] && lane < rows_of_warp && t < 0)
+          for (int c = 0; c < HD / 8; ++c)
+            reinterpret_cast<uint4 *>(out + lane * p.so[2])[c] = make_uint4(0, 0, 0, 0);
       } else {
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->o_full[w], n_o & 1));
         ++n_o;
@@ -400,21 +396,31 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->o_empty[w]);  // the next pair's products may begin
-        // A thread has a row: it writes it sector by sector.
+        // A thread has a row; through shared memory (16-byte chunks placed by
+        // their row, so that both sides meet all banks) the warp writes 128 bytes
+        // of four rows at a time (32 bytes of 32 rows at a time: 1 to 3 % slower).
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-          const uint32_t *f = &o[c / 2][c % 2 * 16];
-          uint32_t v[8];
+        for (int half = 0; half < HD / 64; ++half) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t *f = &o[half * 2 + c / 4][c % 4 * 8];
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = pack2<BF16>(__uint_as_float(f[2 * i]) * inv_l, __uint_as_float(f[2 * i + 1]) * inv_l);
+            sts128(stage + lane * 128 + ((c ^ (lane & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+          }
+          __syncwarp();
+          uint4 v[8];  // rows lane / 8, 4 + lane / 8, ...
+          const int rr = lane >> 3, c = lane & 7;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            v[i] = pack2<BF16>(__uint_as_float(f[2 * i]) * inv_l, __uint_as_float(f[2 * i + 1]) * inv_l);
-          if (!my_row) continue;
-          if (p.wide) {
-            st_global_32(out + c * 16, v);
-          } else {
-            reinterpret_cast<uint4 *>(out)[2 * c] = make_uint4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<uint4 *>(out)[2 * c + 1] = make_uint4(v[4], v[5], v[6], v[7]);
-          }
+            v[i] = lds128(stage + (i * 4 + rr) * 128 + ((c ^ ((i * 4 + rr) & 7)) << 4));
+          uint16_t *to = out + rr * p.so[2] + half * 64 + c * 8;
+#pragma unroll
+          for (int i = 0; i < 8; ++i, to += 4 * p.so[2])
+            if (i * 4 + rr < rows_of_warp) *reinterpret_cast<uint4 *>(to) = v[i];
+          __syncwarp();  // read before it is written again
         }
       }
     }
@@ -727,11 +733,7 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   p.lens = a.lens;
   p.O = static_cast<uint16_t *>(a.O);
-  p.wide = reinterpret_cast<uintptr_t>(a.O) % 32 == 0;
-  for (int i = 0; i < 3; ++i) {
-    p.so[i] = a.so[i];
-    p.wide = p.wide && a.so[i] % 16 == 0;
-  }
+  for (int i = 0; i < 3; ++i) p.so[i] = a.so[i];
   p.Hq = a.Hq;
   p.Hkv = a.Hkv;
   p.Nq = a.Nq;
