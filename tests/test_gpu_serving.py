@@ -200,6 +200,21 @@ def test_window_pairs_of_tiles(gpu, shape, d, t):
                  tokens_first=d == 64, seed=Nq + Hq)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 200), (520, 0)])
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("d", [64, 128])
+def test_window_halves_of_keys(gpu, d, t, window, sinks):
+    """Few row tiles, whose keys are shared out: one to nine key tiles, odd and even, sequences that
+    end within a tile and on its border, scores that make one half's share vanish."""
+    B, Hq, N = 8, 2, 1100
+    assert (N + 127) // 128 * Hq * B <= 148
+    rows = [0, 1, 127, 128, 300, 511, 512, 639, 640, 800, 896, 1023, 1024, 1098, 1099]
+    _window_case(gpu, t, B, Hq, 1, N, N, d, window, sinks, lens=[1100, 1025, 1024, 897, 640, 385, 129, 3],
+                 rows=rows, seed=d + window)
+    _window_case(gpu, t, 4, Hq, 2, N, N + 333, d, window, sinks, q_scale=20.0, rows=rows,
+                 tokens_first=True, seed=d + window + 1)
+
+
 def test_window_matches_flash_fwd(gpu):
     """Without a window it is the causal vc_flash_fwd."""
     B, H, N, d = 2, 3, 500, 128

@@ -40,6 +40,11 @@
 // walks the union of its two tiles' key tiles - those of the sinks, then from
 // the window's lower edge to the diagonal - and each row tile skips the ones
 // it does not see. Only tiles on an edge are masked.
+//
+// Few row tiles (SPLIT): a step takes as long with one tile as with two, because
+// a tile's scores, softmax and products follow one another. So a CTA takes one
+// row tile and each half of it takes half of its keys, with its own S, O, maximum
+// and sum; at the end the first half's warps read both O from TMEM.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -76,7 +81,9 @@ struct KeyTiles {
 };
 
 // A pair of row tiles of the query heads that share a K/V head, and the key
-// tiles of their union: [0, sink), then [lo, hi).
+// tiles of their union: [0, sink), then [lo, hi). Or (SPLIT) one row tile, whose
+// key tiles the two halves of the CTA share: they take them in turns, one the
+// lower half of the list, the other, which has the last turn, the upper.
 struct Work {
   int valid;                   // 0: the queue is empty
   int b, kvh, n;               // n: tokens of the sequence
@@ -84,10 +91,15 @@ struct Work {
   KeyTiles kt[2];
   int lo, hi, sink, total;
   int clean;                   // V's rows from n on are zeroed in the last tile
-  int chained;                 // K(0) shares the stage of the last pair's last V
+  int chained;                 // K(0) shares the stage of the last pair's last V (pairs only)
   int stage0, n_live, n_clean; // stage of K(0); pairs with keys, cleaned tiles before this one
-  __device__ __forceinline__ int tile_of(int u) const { return u < sink ? u : lo + (u - sink); }
 };
+// Key tile of step u of a list [0, sink), [lo, ...) of `total`.
+template <bool SPLIT>
+__device__ __forceinline__ int tile_of(int u, int total, int sink, int lo) {
+  const int i = !SPLIT ? u : (u >> 1) + ((u ^ (total - 1)) & 1 ? 0 : total >> 1);
+  return i < sink ? i : lo + (i - sink);
+}
 
 struct __align__(16) WindowBarriers {
   uint4 answer;  // of the grid's queue
@@ -101,6 +113,8 @@ struct __align__(16) WindowBarriers {
   uint64_t s_full[2];
   uint64_t p_full[2][2];
   uint64_t o_full[2], o_empty[2];
+  uint64_t stats_full[4], stats_empty[4];  // of the quadrants of a split row tile
+  float2 stats[BQ];                        // maxima and sums of its second half
   uint32_t tmem_base;
 };
 
@@ -123,18 +137,19 @@ struct WindowParams {
   uint16_t *O;
   int64_t so[3];
   int Hq, Hkv, Nq, Nk, window, sinks;
-  int per_cta;  // row tiles that a CTA takes at a time: 2, or 1
+  int items, slices;  // pairs (split: row tiles) of a slice (a sequence's K/V head); slices
   float scale_log2;
 };
 
 // Order of the grid: groups of K/V slices, the last rows (with the most keys)
 // of every slice of a group first.
-__device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Work &k) {
-  const int lin = y * gridDim.x + x, per = kOrderGroup * gridDim.x;
-  const int g = lin / per, first = g * kOrderGroup;
-  const int gsz = min(kOrderGroup, (int)gridDim.y - first);
-  const int r = lin - g * per;
-  const int pair = gridDim.x - 1 - r / gsz, slice = first + r % gsz;
+template <bool SPLIT>
+__device__ __forceinline__ void work_of(const WindowParams &p, int item, Work &k) {
+  const int per = kOrderGroup * p.items;
+  const int g = item / per, first = g * kOrderGroup;
+  const int gsz = min(kOrderGroup, p.slices - first);
+  const int r = item - g * per;
+  const int pair = p.items - 1 - r / gsz, slice = first + r % gsz;
   const int group = p.Hq / p.Hkv;
   const int shift = p.Nk - p.Nq;  // position of row 0
   const int b = slice / p.Hkv, kvh = slice - b * p.Hkv;
@@ -144,13 +159,13 @@ __device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Wor
   int count[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int unit = p.per_cta * pair + w;
+    const int unit = SPLIT ? pair : 2 * pair + w;
     const int row0 = unit / group * BQ;
     // Positions of the rows that are computed: the last one has the most keys.
     const int t_first = max(row0 + shift, 0);
     const int t_last = min(min(row0 + BQ, p.Nq) - 1 + shift, n - 1);
     kt[w] = {0, 0, 0};
-    const bool exists = w < p.per_cta && unit < units;
+    const bool exists = unit < units;
     if (exists && t_last >= t_first) {
       kt[w].hi = t_last / BKV + 1;
       if (p.window > 0) {
@@ -161,8 +176,8 @@ __device__ __forceinline__ void work_of(const WindowParams &p, int x, int y, Wor
     count[w] = kt[w].count();
     k.row0[w] = row0;
     k.head[w] = kvh * group + unit % group;
-    k.exists[w] = exists;
-    k.count[w] = count[w];
+    k.exists[w] = exists && !(SPLIT && w);
+    k.count[w] = !SPLIT ? count[w] : w ? count[w] / 2 : (count[w] + 1) / 2;
     k.kt[w] = kt[w];
   }
   const int lo = count[0] && count[1] ? min(kt[0].lo, kt[1].lo) : count[0] ? kt[0].lo : kt[1].lo;
@@ -191,7 +206,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-template <int HD, bool BF16>
+template <int HD, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 flash_window_kernel(const __grid_constant__ WindowParams p) {
   using L = WindowSmem<HD>;
@@ -226,6 +241,11 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     }
     fence_barrier_init();
   }
+  if (threadIdx.x == 32)
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bars->stats_full[i], 1);
+      mbar_init(&bars->stats_empty[i], 1);
+    }
   if (warp == 9) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
@@ -263,18 +283,20 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     const uint32_t o_col = tmem + lane_off + 256 + w * 128;
     const uint32_t stage = smem_u32(smem + L::kOut) + warp * 4096;
     int n_s = 0, n_o = 0;  // S tiles and O tiles so far
+    int n_o1 = 0, n_split = 0;  // O tiles of the second half, exchanges of statistics
     bool ok = true;
     for (; wait_work(round) && bars->work[round & 1].valid; done()) {
       const Work &k = bars->work[round & 1];
       const KeyTiles mine = k.kt[w];
       const int count = k.count[w], row0 = k.row0[w], head = k.head[w];
       const int total = k.total, lo = k.lo, sink = k.sink, n = k.n;
+      const bool both = SPLIT && total > 1;  // a split tile of which both halves have keys
       const int t_first = row0 + p.Nk - p.Nq, t = t_first + row;  // positions
       float m_run = -INFINITY;  // running max of scale_log2 * s
       float l_run = 0.0f;
       bool first = true;
-      for (int u = 0; u < total; ++u) {
-        const int tile = u < sink ? u : lo + (u - sink);
+      for (int u = SPLIT ? w : 0; u < total; u += 1 + SPLIT) {
+        const int tile = tile_of<SPLIT>(u, total, sink, lo);
         if (!mine.has(tile)) continue;
         if (!mbar_wait(&bars->s_full[w], n_s & 1)) ok = false;
         ++n_s;
@@ -383,19 +405,57 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         if (k.exists[w] && lane < rows_of_warp && t < 0)
           for (int c = 0; c < HD / 8; ++c)
             reinterpret_cast<uint4 *>(out + lane * p.so[2])[c] = make_uint4(0, 0, 0, 0);
+      } else if (both && w == 1) {
+        // The other half's warps write the rows.
+        ++n_o;
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->stats_empty[quad], (n_split & 1) ^ 1));
+        if (!ok) break;
+        bars->stats[row] = make_float2(m_run, l_run);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->stats_full[quad]);
+        ++n_split;
       } else {
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->o_full[w], n_o & 1));
         ++n_o;
         if (!ok) break;
+        float f0 = 1.0f, f1 = 1.0f;  // factors of the halves
+        if (both) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->stats_full[quad], n_split & 1) &&
+                                           mbar_wait(&bars->o_full[1], n_o1 & 1));
+          ++n_split;
+          if (!ok) break;
+          const float2 other = bars->stats[row];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->stats_empty[quad]);
+          // A side without a visible key holds zeros (or NaN, which stays).
+          const float m = fmaxf(m_run, other.x);
+          if (m_run != -INFINITY) f0 = ex2_approx(m_run - m);
+          if (other.x != -INFINITY) f1 = ex2_approx(other.x - m);
+          l_run = l_run * f0 + other.y * f1;
+        }
         tc_fence_after();
         const float inv_l = l_run != 0.0f ? 1.0f / l_run : 0.0f;
         uint32_t o[HD / 32][32];
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) tmem_ld32(o_col + c * 32, o[c]);
         tmem_ld_wait();
+        if (both) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o1[32];
+            tmem_ld32(o_col + 128 + c * 32, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              o[c][x] = __float_as_uint(__uint_as_float(o[c][x]) * f0 + __uint_as_float(o1[x]) * f1);
+          }
+        }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->o_empty[w]);  // the next pair's products may begin
+        if (lane == 0) {  // the next pair's products may begin
+          mbar_arrive(&bars->o_empty[w]);
+          if (both) mbar_arrive(&bars->o_empty[1]);
+        }
         // A thread has a row; through shared memory (16-byte chunks placed by
         // their row, so that both sides meet all banks) the warp writes 128 bytes
         // of four rows at a time (32 bytes of 32 rows at a time: 1 to 3 % slower).
@@ -423,13 +483,14 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
           __syncwarp();  // read before it is written again
         }
       }
+      n_o1 += k.count[1] > 0;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 10) {
       // ------------------------------------------------ scheduler
       if (lane == 0) {
-        int x = blockIdx.x, y = blockIdx.y;
+        int x = blockIdx.x, y = 0;
         int stage = 0, n_live = 0, n_clean = 0;
         bool live = false;  // the last pair had keys
         for (int r = 0;; ++r) {
@@ -445,8 +506,8 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
           }
           k.valid = have;
           if (have) {
-            work_of(p, x, y, k);
-            k.chained = live && k.total > 0;
+            work_of<SPLIT>(p, x, k);
+            k.chained = !SPLIT && live && k.total > 0;
             live = k.total > 0;
             if (live) {
               // Its K(0) joins the last pair's last V, or begins a stage.
@@ -454,7 +515,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
               k.n_live = n_live++;
               k.n_clean = n_clean;
               n_clean += k.clean;
-              stage = k.stage0 + k.total + 1;
+              stage = k.stage0 + k.total + 1 + SPLIT;
             }
           } else {
             k.chained = 0;
@@ -490,11 +551,13 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         }
         return true;
       };
+      auto tile = [](const Work &k, int u) { return tile_of<SPLIT>(u, k.total, k.sink, k.lo); };
       for (; ok && wait_work(round) && bars->work[round & 1].valid; done()) {
         const Work &k = bars->work[round & 1], &next = bars->work[(round + 1) & 1];
         if (k.total == 0) continue;
+        constexpr int ahead = 1 + SPLIT;  // steps that K is ahead of V
         if (lane == 0) {
-          if (!k.chained) ok = load_stage(k.stage0, nullptr, 0, &k, k.tile_of(0));
+          if (!k.chained) ok = load_stage(k.stage0, nullptr, 0, &k, tile(k, 0));
           ok = ok && mbar_wait(&bars->q_empty, (k.n_live & 1) ^ 1);
           if (ok) {
             mbar_arrive_expect_tx(&bars->q_full, ((k.count[0] > 0) + (k.count[1] > 0)) * L::kTile);
@@ -507,14 +570,15 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
                               k.b, &bars->q_full);
               }
           }
-          for (int u = 0; ok && u + 1 < k.total; ++u)
-            ok = load_stage(k.stage0 + u + 1, &k, k.tile_of(u), &k, k.tile_of(u + 1));
+          for (int u = 1 - ahead; ok && u + 1 < k.total; ++u)
+            ok = load_stage(k.stage0 + u + ahead, u >= 0 ? &k : nullptr, tile(k, u),
+                            u + ahead < k.total ? &k : nullptr, tile(k, u + ahead));
         }
         ok = __shfl_sync(0xffffffffu, ok, 0) && wait_work(round + 1);
         if (ok && lane == 0) {
           const bool chain = next.valid && next.chained;
-          ok = load_stage(k.stage0 + k.total, &k, k.tile_of(k.total - 1), chain ? &next : nullptr,
-                          chain ? next.tile_of(0) : 0);
+          ok = load_stage(k.stage0 + k.total - 1 + ahead, &k, tile(k, k.total - 1), chain ? &next : nullptr,
+                          chain ? tile(next, 0) : 0);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
       }
@@ -536,7 +600,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         if (!k.clean) continue;
         // The issuer has seen the stage arrive; it stays until the issuer goes on
         // (a stage's own barrier may be phases behind when this warp comes here).
-        const int s = k.stage0 + k.total, st = s % kStages;
+        const int s = k.stage0 + k.total + SPLIT, st = s % kStages;
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_dirty, k.n_clean & 1) &&
                                          mbar_wait(&bars->kv_full[st], (s / kStages) & 1));
         if (!ok) break;
@@ -585,34 +649,34 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
           left[w] = uni(k.count[w]);
         }
         const int lo = uni(k.lo), sink = uni(k.sink), stage0 = uni(k.stage0);
-        auto tile_of = [&](int u) { return u < sink ? u : lo + (u - sink); };
         bool begun[2] = {false, false};
-        int u = uni(k.chained) ? 0 : -1;
+        int u = uni(k.chained) ? 0 : -1 - SPLIT;
         if (u < 0) wait(&bars->q_full, uni(k.n_live) & 1);
         // Step u in stage s = stage0 + u + 1: the products of V(u), and the scores
         // of K(u + 1), which after the last step is the next pair's first. u = -1:
-        // scores only.
+        // scores only. (A split tile's steps belong to its halves in turns, and K
+        // is two steps ahead: u begins at -2.)
 #pragma unroll 1
         for (; ok && u < total; ++u) {
           const bool last = u + 1 == total;
-          const int tile = tile_of(u), after = tile_of(u + 1);
+          const int tile = tile_of<false>(u, total, sink, lo), after = tile_of<false>(u + 1, total, sink, lo);
           bool pv[2], sc[2];  // products and scores to issue
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            pv[w] = u >= 0 && kt[w].has(tile);
-            sc[w] = kt[w].has(after);
+            pv[w] = u >= 0 && (SPLIT ? (u & 1) == w : kt[w].has(tile));
+            sc[w] = SPLIT ? (u & 1) == w && u + 2 < total : kt[w].has(after);
           }
-          bool chain = false, q_free = u + 2 == total;
+          bool chain = false, q_free = u + 2 + SPLIT == total;
           if (last) {
             ok = wait_work(round + 1);
             if (!ok) break;
             chain = uni(next.valid && next.chained);
             q_free = chain && uni(next.total) == 1;
-            const int t0 = next.tile_of(0);
+            const int t0 = tile_of<false>(0, next.total, next.sink, next.lo);
             sc[0] = uni(chain && next.kt[0].has(t0));
             sc[1] = uni(chain && next.kt[1].has(t0));
           }
-          const int s = stage0 + u + 1, st = s % kStages;
+          const int s = stage0 + u + 1 + SPLIT, st = s % kStages;
           const uint32_t v_lo = dv_lo + (2 * st * L::kTile >> 4), k_lo = dq_lo + ((3 + 2 * st) * L::kTile >> 4);
           wait(&bars->kv_full[st], (s / kStages) & 1);
           if (last && uni(k.clean)) {
@@ -693,8 +757,8 @@ bool make_map(CUtensorMap *map, bool bf16, const void *base, int B, int H, int N
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, bool BF16>
-cudaError_t launch_typed(const WindowParams &p, dim3 grid, cudaStream_t stream) {
+template <int HD, bool BF16, bool SPLIT>
+cudaError_t launch_typed(const WindowParams &p, int grid, cudaStream_t stream) {
   static uint64_t configured = 0;  // devices whose smem attribute is set
   static std::mutex mu;
   int dev = 0;
@@ -702,7 +766,7 @@ cudaError_t launch_typed(const WindowParams &p, dim3 grid, cudaStream_t stream) 
   {
     std::lock_guard<std::mutex> lk(mu);
     if (dev >= 64 || !(configured & (1ull << dev))) {
-      cudaError_t e = cudaFuncSetAttribute(flash_window_kernel<HD, BF16>,
+      cudaError_t e = cudaFuncSetAttribute(flash_window_kernel<HD, BF16, SPLIT>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)WindowSmem<HD>::kBytes);
       if (e != cudaSuccess) return e;
@@ -710,7 +774,7 @@ cudaError_t launch_typed(const WindowParams &p, dim3 grid, cudaStream_t stream) 
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = WindowSmem<HD>::kBytes;
   cfg.stream = stream;
@@ -719,7 +783,12 @@ cudaError_t launch_typed(const WindowParams &p, dim3 grid, cudaStream_t stream) 
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, flash_window_kernel<HD, BF16>, p);
+  return cudaLaunchKernelEx(&cfg, flash_window_kernel<HD, BF16, SPLIT>, p);
+}
+
+template <int HD, bool BF16>
+cudaError_t launch_any(const WindowParams &p, int grid, bool split, cudaStream_t stream) {
+  return split ? launch_typed<HD, BF16, true>(p, grid, stream) : launch_typed<HD, BF16, false>(p, grid, stream);
 }
 
 }  // namespace
@@ -743,16 +812,19 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   p.scale_log2 = a.scale_log2;
   const int64_t units = ((int64_t)a.Nq + BQ - 1) / BQ * (a.Hq / a.Hkv);
   if (units * a.B * a.Hkv > INT32_MAX / kOrderGroup) return cudaErrorInvalidValue;
-  // One row tile a CTA while every tile can have an SM of its own: a step then
-  // takes 1.5 us instead of 1.9 (8 heads x 1024 tokens, 64 tiles: 17.7 us
-  // against 21.7; 8 x 2048, 128 tiles: 29.9 against 36.2). With more tiles than
-  // SMs two share the loads and the tensor cores' gaps (256 tiles: 36.0 us
-  // against 42.0; 1024: 85 against 117).
-  p.per_cta = units * a.B * a.Hkv <= sm_count_current() ? 1 : 2;
-  const dim3 grid((unsigned)((units + p.per_cta - 1) / p.per_cta), a.B * a.Hkv);
+  p.slices = a.B * a.Hkv;
+  // Two row tiles a CTA share the loads and fill the tensor cores' gaps. While
+  // every row tile can have an SM of its own, two halves of its keys do: 8 heads
+  // x 512 tokens 10.6 us (with one row tile a CTA, whose steps follow one another,
+  // 11.4), x 1024 14.7 (17.6), x 2048 22.9 (29.4), 2 x 8192 of d 64 57.5 (85).
+  // With more row tiles than SMs it is the other way round (32 x 2048, 512 tiles:
+  // 57 us split, 51 in pairs), or the same (256 tiles: 35.5 and 35.8).
+  const bool split = units * p.slices <= sm_count_current();
+  p.items = (int)(split ? units : (units + 1) / 2);
+  const int grid = p.items * p.slices;
   if (a.d == 64)
-    return bf16 ? launch_typed<64, true>(p, grid, stream) : launch_typed<64, false>(p, grid, stream);
-  return bf16 ? launch_typed<128, true>(p, grid, stream) : launch_typed<128, false>(p, grid, stream);
+    return bf16 ? launch_any<64, true>(p, grid, split, stream) : launch_any<64, false>(p, grid, split, stream);
+  return bf16 ? launch_any<128, true>(p, grid, split, stream) : launch_any<128, false>(p, grid, split, stream);
 }
 
 }  // namespace vcb
