@@ -8,8 +8,8 @@
 // Bound: HBM, 2 d bytes per visible key and K/V head, each read once; the
 // query heads that share a K/V head are the columns of one matrix product.
 // Measured (head dim 128, 8 K/V heads of 4 query heads): 32 sequences of up to
-// 16384 tokens 105 us, 5.86 TB/s, 0.90 of the copy rate; 64 of up to 16384
-// (4 K/V heads) through a window of 4096 53 us, 4.9 TB/s. Of a call's time about
+// 16384 tokens 104 us, 5.9 TB/s, 0.90 of the copy rate; 64 of up to 16384
+// (4 K/V heads) through a window of 4096 52 us, 5.0 TB/s. Of a call's time about
 // 9 us do not shrink with the work: lengths, page numbers, scales and the first
 // codes come one after the other (5 us), and at the end the warps' and the
 // blocks' results are joined (4 us).
@@ -26,7 +26,9 @@
 // A warp takes 32 of a tile's 128 keys, through a ring of its own that TMA
 // fills: boxes of 16 or 32 rows of the page's codes, swizzled so that the
 // reads below meet no bank twice. Warps of a block meet only where an item
-// ends. Rows that the mask hides arrive too; their scores become minus
+// ends: there each joins a quarter of the results, while the next item's queries
+// are on their way (two warps, then one, and the queries after that: 256 sequences
+// of up to 500 tokens took 63.6 us instead of 55.0). Rows that the mask hides arrive too; their scores become minus
 // infinity and their values zero, whatever they hold. Per 16 keys, with
 // m16n8k16 fp16 products and fp32 accumulators:
 //   S^T = K Q^T   A = the codes as fp16 (exact), rows keys; B = q. The order of
@@ -57,9 +59,9 @@ constexpr int kTile = 128;     // keys per tile
 constexpr int kWarps = 4;      // 32 keys each
 constexpr int kThreads = kWarps * 32;
 // Two blocks with 16 KB of ring per warp: 32 sequences of up to 16384 tokens
-// 105 us, one of 32000 17.6 us. Three: 109 and 20.6 us (more parts to join),
-// though 64 sequences of up to 700 tokens take 23.3 us instead of 25.4; one
-// block of 8 warps: 109, 14.5 and 31.8 us.
+// 105 us, one of 32000 17.6 us, 64 of up to 700 25.4 us (104, 17 and 23.0 since).
+// Three: 109, 20.6 (more parts to join) and 23.3 us; one block of 8 warps: 109,
+// 14.5 and 31.8 us.
 constexpr int kBlocksPerSm = 2;
 constexpr int kMaxHeads = 16;  // query heads of an item
 constexpr float kLazy = 8.0f;  // log2 units
@@ -162,7 +164,7 @@ struct Smem {
   static constexpr int kBars = kMetas + kWarps * kStages * 32;
   static constexpr int kMerge = kBars + ((kWarps * kStages * 8 + 15) & ~15);
   static constexpr int kMergeWarp = 32 * (D * NT / 4 + 4 * NT);  // floats a warp hands over
-  static constexpr int kBytes = kMerge + 2 * kMergeWarp * 4 + 1024;  // the ring 1024-byte aligned
+  static constexpr int kBytes = kMerge + kWarps * kMergeWarp * 4 + 1024;  // the ring 1024-byte aligned
 };
 struct alignas(16) Meta {
   float k_scale[2], v_scale[2];  // of the halves
@@ -506,20 +508,16 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
   uint32_t phase = 0;
   bool ok = true;
 
-  int stage = 0;
-  for (int64_t at_tile = t0; at_tile < t1;) {
-    // ---- one item: its queries
-    const int head = cur.item / p.groups, grp = cur.item % p.groups;
-    const int h0 = head * p.group + grp * NH;  // first query head
-    const int nh = min(NH, p.group - grp * NH);
-    uint32_t q[NT][D / 16][2];
-    float mult[NT][2];  // of the scores of this thread's two columns
+  // Queries of an item, as they are.
+  uint32_t q[NT][D / 16][2];
+  auto load_q = [&](const Cursor &c) {
+    const int h0 = c.item / p.groups * p.group + c.item % p.groups * NH;
+    const int nh = min(NH, p.group - c.item % p.groups * NH);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool have = nt * 8 + r < nh;
-      const uint16_t *src = static_cast<const uint16_t *>(p.Q) + cur.b * p.q_stride +
+      const uint16_t *src = static_cast<const uint16_t *>(p.Q) + c.b * p.q_stride +
                             (int64_t)(h0 + nt * 8 + (have ? r : 0)) * D + t * 16;
-      float inv = 1.0f;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ks += 2) {
         const uint4 w = have ? *reinterpret_cast<const uint4 *>(src + (ks / 4) * 64 + (ks % 4) * 4)
@@ -529,6 +527,19 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
         q[nt][ks + 1][0] = w.z;
         q[nt][ks + 1][1] = w.w;
       }
+    }
+  };
+  load_q(cur);
+  int stage = 0;
+  for (int64_t at_tile = t0; at_tile < t1;) {
+    // ---- one item: its queries
+    const int grp = cur.item % p.groups;
+    const int h0 = cur.item / p.groups * p.group + grp * NH;  // first query head
+    const int nh = min(NH, p.group - grp * NH);
+    float mult[NT][2];  // of the scores of this thread's two columns
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float inv = 1.0f;
       if constexpr (BF16) {
         uint32_t top = 0;  // largest magnitude's bits
 #pragma unroll
@@ -728,8 +739,20 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       issue(mine);
     }
 
-    // ---- the warps' results joined: 2 and 3 into 0 and 1, then 1 into 0, each
-    // thread's registers through shared memory to the same lane of the other.
+    // ---- the next item's queries are on their way while this one is joined
+    const int64_t item0 = at_tile - cur.tile, item1 = item0 + cur.tiles.count;
+    const bool whole = item0 >= t0 && item1 <= t1;
+    const int slot_of_mine = item0 <= t0 ? 0 : 1;
+    uint16_t *const out = static_cast<uint16_t *>(p.O) + cur.b * p.o_stride + (int64_t)h0 * D;
+    at_tile += n;
+    cur.tile += n;
+    if (at_tile < t1) {
+      next_item(cur, p);
+      load_q(cur);
+    }
+
+    // ---- the warps' results joined, through shared memory: each warp takes a
+    // quarter of the fragments, from the same lanes of all warps in order.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -739,86 +762,72 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
         l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 16);
       }
     constexpr int kFrags = D / 16 * NT;  // float4 of O per thread
+    float4 *const mine = reinterpret_cast<float4 *>(merge + warp * S::kMergeWarp) + lane;
 #pragma unroll
-    for (int half = kWarps / 2; half; half >>= 1) {
-      float4 *const buf = reinterpret_cast<float4 *>(merge + (warp % half) * S::kMergeWarp) + lane;
-      if (warp >= half && warp < 2 * half) {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            buf[(nt * (D / 16) + i) * 32] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
-          buf[(kFrags + nt) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
-        }
-      }
-      __syncthreads();
-      if (warp < half) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float4 ml = buf[(kFrags + nt) * 32];
-          float fa[2], fb[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float ma = m[nt][x], mb = x ? ml.y : ml.x, mx = fmaxf(ma, mb);
-            // A side without a visible key holds zeros (or NaN, which stays).
-            fa[x] = ma == -INFINITY ? 1.0f : ex2_approx(ma - mx);
-            fb[x] = mb == -INFINITY ? 1.0f : ex2_approx(mb - mx);
-            m[nt][x] = mx;
-            l[nt][x] = l[nt][x] * fa[x] + (x ? ml.w : ml.z) * fb[x];
-          }
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const float4 y = buf[(nt * (D / 16) + i) * 32];
-            o[nt][i][0] = o[nt][i][0] * fa[0] + y.x * fb[0];
-            o[nt][i][1] = o[nt][i][1] * fa[1] + y.y * fb[1];
-            o[nt][i][2] = o[nt][i][2] * fa[0] + y.z * fb[0];
-            o[nt][i][3] = o[nt][i][3] * fa[1] + y.w * fb[1];
-          }
-        }
-      }
-      __syncthreads();
+      for (int i = 0; i < D / 16; ++i)
+        mine[(nt * (D / 16) + i) * 32] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+      mine[(kFrags + nt) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
     }
-    const int64_t item0 = at_tile - cur.tile, item1 = item0 + cur.tiles.count;
-    const bool whole = item0 >= t0 && item1 <= t1;
-    const int slot_of_mine = item0 <= t0 ? 0 : 1;
-    uint16_t *const out = static_cast<uint16_t *>(p.O) + cur.b * p.o_stride + (int64_t)h0 * D;
-    float4 *const my_slot =
-        reinterpret_cast<float4 *>(p.slots + ((size_t)blockIdx.x * 2 + slot_of_mine) * kSlotFloats);
-    if (warp == 0) {
+    __syncthreads();
+    {
+      constexpr int kShare = kFrags / kWarps;
+      const int nt = warp * kShare / (D / 16);  // of all of them
+      const float4 *const from = reinterpret_cast<const float4 *>(merge) + lane;
+      constexpr int kStep = S::kMergeWarp / 4;
+      float4 ml[kWarps];
+      float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, f[kWarps][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int w = 0; w < kWarps; ++w) {
+        ml[w] = from[w * kStep + (kFrags + nt) * 32];
+        mx[0] = fmaxf(mx[0], ml[w].x);
+        mx[1] = fmaxf(mx[1], ml[w].y);
+      }
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const float4 v = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
-          if (whole)
-            write_fragment<D, BF16>(out, nh, lane, nt, i, v, l[nt][0], l[nt][1]);
-          else
-            __stcg(my_slot + (nt * (D / 16) + i) * 32 + lane, v);
+      for (int w = 0; w < kWarps; ++w) {
+        // A side without a visible key holds zeros (or NaN, which stays).
+        f[w][0] = ml[w].x == -INFINITY ? 1.0f : ex2_approx(ml[w].x - mx[0]);
+        f[w][1] = ml[w].y == -INFINITY ? 1.0f : ex2_approx(ml[w].y - mx[1]);
+        sum[0] += ml[w].z * f[w][0];
+        sum[1] += ml[w].w * f[w][1];
+      }
+      float4 *const my_slot =
+          reinterpret_cast<float4 *>(p.slots + ((size_t)blockIdx.x * 2 + slot_of_mine) * kSlotFloats);
+#pragma unroll
+      for (int j = 0; j < kShare; ++j) {
+        const int at = warp * kShare + j;
+        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 y = from[w * kStep + at * 32];
+          v.x += y.x * f[w][0];
+          v.y += y.y * f[w][1];
+          v.z += y.z * f[w][0];
+          v.w += y.w * f[w][1];
         }
-        // The maxima and sums of a slot: [column] pairs behind its fragments.
-        if (!whole && r == 0) {
-          float2 *ml = reinterpret_cast<float2 *>(my_slot + kFrags * 32) + nt * 8 + 2 * t;
-          __stcg(ml, make_float2(m[nt][0], l[nt][0]));
-          __stcg(ml + 1, make_float2(m[nt][1], l[nt][1]));
-        }
+        if (whole)
+          write_fragment<D, BF16>(out, nh, lane, nt, at % (D / 16), v, sum[0], sum[1]);
+        else
+          __stcg(my_slot + at * 32 + lane, v);
+      }
+      // The maxima and sums of a slot: [column] pairs behind its fragments.
+      if (!whole && r == 0 && warp * kShare % (D / 16) == 0) {
+        float2 *to = reinterpret_cast<float2 *>(my_slot + kFrags * 32) + nt * 8 + 2 * t;
+        __stcg(to, make_float2(mx[0], sum[0]));
+        __stcg(to + 1, make_float2(mx[1], sum[1]));
       }
     }
+    __syncthreads();  // the merge buffer is free again, the block's stores come before the arrival
     // A part is counted in at once, but its join, where it falls to this block,
     // waits for the block's own work, which may be what others wait for.
-    if (!whole && warp == 0) {
-      __syncwarp();  // the warp's stores come before the arrival
-      if (lane == 0) {
-        Part &part = sh_parts[at_tile + n < t1 ? 0 : 1];
-        part.join = join_of(split, item0, item1);
-        part.out = out;
-        part.nh = nh;
-        part.before = arrive(&p.counters[part.join.lead >> 1].group[part.join.lead & 1]);
-      }
+    if (!whole && tid == 0) {
+      Part &part = sh_parts[at_tile < t1 ? 0 : 1];
+      part.join = join_of(split, item0, item1);
+      part.out = out;
+      part.nh = nh;
+      part.before = arrive(&p.counters[part.join.lead >> 1].group[part.join.lead & 1]);
     }
-    __syncthreads();  // the merge buffer is free again
-    at_tile += n;
-    cur.tile += n;
-    if (at_tile < t1) next_item(cur, p);
   }
   __syncthreads();
 #pragma unroll 1
