@@ -1,0 +1,75 @@
+"""The cache attention at the ends of its documented range: value scales, scores
+and lengths, against closed forms and the float64 forms of kv8_plain.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_plain as plain
+from test_gpu_serving import Cache, _done, _dt, _f64, _ints
+
+pytestmark = pytest.mark.gpu
+
+
+def _attn_call(gpu, c, q, table, lens, scale, window=0, sinks=0):
+    """One call over a cache as it is; q [B][Hq][d]."""
+    B, Hq = q.shape[:2]
+    o = torch.full_like(q, 7.0)
+    ws = torch.zeros(gpu.kv8_attn_workspace(c.handle, B, Hq)[1], dtype=torch.uint8, device="cuda")
+    assert gpu.kv8_attn(c.handle, q, o, _ints(table), table.shape[1], _ints(lens), B, Hq, scale,
+                        _dt(gpu, q.dtype), ws, ws.numel(), window=window, sinks=sinks) == 0
+    _done(gpu)
+    return _f64(o)
+
+
+def _code(x):
+    return int(plain.to_e4m3(np.array([float(x)]))[0])
+
+
+@pytest.mark.parametrize("Hq,d", [(1, 128), (9, 64), (20, 128)])
+@pytest.mark.parametrize("n", [32, 128, 272, 5000, 90000])
+@pytest.mark.parametrize("big,small", [(27, -100), (119, -100), (17, None), (119, None), (0, -100)])
+def test_attn_value_scales_do_not_move_the_weights(gpu, big, small, n, Hq, d):
+    """Equal scores over pages whose value scales are up to 2^219 apart (None: a page of scale 0, as
+    memory comes): the pages with the small scale hold zeros, and their keys' share of the sum counts.
+    One page holds ones: the first, the second, one of another warp, the last."""
+    P = 16
+    pages = -(-n // P)
+    c = Cache(gpu, pages, 1, P, d)
+    table = np.random.default_rng(n).permutation(pages).astype(np.int32)[None]
+    c.k.fill_(_code(1.0))
+    c.ks.fill_(2.0 ** -3)
+    q = torch.randn(1, Hq, d, device="cuda").bfloat16()
+    for at in sorted({0, 1, 2, 4, 9, pages - 1} & set(range(pages))):
+        c.v.fill_(0)
+        c.vs.fill_(0.0 if small is None else 2.0 ** small)
+        c.v[table[0, at]] = _code(1.0)
+        c.vs[table[0, at]] = 2.0 ** big
+        # All weights are 1 / n: the output's rounding and the weights', all values of one sign.
+        want = 2.0 ** big * min(P, n - at * P) / n
+        got = _attn_call(gpu, c, q, table, [n], 0.1)
+        assert (np.abs(got - want) <= want * (2.0 ** -8 + 2.0 ** -10)).all(), (at, got.min() / want, got.max() / want)
+
+
+@pytest.mark.parametrize("exp", [119, 0, -100])
+@pytest.mark.parametrize("n,heavy", [(600, 0), (600, 20), (40000, 5), (40000, 2499)])
+def test_attn_lower_scores_keep_their_share(gpu, n, heavy, exp):
+    """16 keys 10 log2 units above all others, at the ends of the range of value scales: the others are
+    a good part of the sum."""
+    P, d = 16, 64
+    pages = -(-n // P)
+    c = Cache(gpu, pages, 1, P, d)
+    table = np.random.default_rng(n).permutation(pages).astype(np.int32)[None]
+    c.k.fill_(0)
+    c.k[:, :, :, 0] = _code(-2.0)
+    c.k[table[0, heavy], :, :, 0] = _code(8.0)
+    c.v.fill_(0)
+    c.v[table[0, heavy]] = _code(1.0)
+    c.vs.fill_(2.0 ** exp)
+    q = torch.zeros(1, 3, d, device="cuda").bfloat16()
+    q[:, :, 0] = 1.0
+    want = 2.0 ** exp * P / (P + (n - P) * 2.0 ** -10)
+    got = _attn_call(gpu, c, q, table, [n], 1.0)
+    # The sum's n terms are exact powers of two; the output's rounding and the weights'.
+    assert (np.abs(got - want) <= want * (2.0 ** -8 + 2.0 ** -10)).all(), got / want

@@ -40,8 +40,13 @@
 // but for elements 2^-28 below the row's largest). The value scale of a page
 // enters the weights: p' = 2^(s + log2 v_scale - m), m the running maximum of
 // s + log2 v_scale, so that the weights stay within fp16 whatever the scales
-// are, while the sum of the softmax takes 2^(s - m). The maximum follows
-// lazily: it moves when a value exceeds it by more than 2^8.
+// are. What a weight below 2^-25 of the largest would add, less than 2^-16 of a
+// unit of the codes that have the largest, is left out (their half step is 2^-10
+// at least). The sum of the softmax has a maximum of its own, that of s: relative
+// to m its terms would lie between 2^-119 and 2^110, and the factor between two
+// such sums is not an fp32 number. Both maxima follow lazily: they move when a
+// value exceeds its own by more than 2^8. Where the warps' results are joined,
+// products and sums come to one reference, see there.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -163,7 +168,7 @@ struct Smem {
   static constexpr int kMetas = kRing;       // of every stage
   static constexpr int kBars = kMetas + kWarps * kStages * 32;
   static constexpr int kMerge = kBars + ((kWarps * kStages * 8 + 15) & ~15);
-  static constexpr int kMergeWarp = 32 * (D * NT / 4 + 4 * NT);  // floats a warp hands over
+  static constexpr int kMergeWarp = 32 * (D * NT / 4 + 6 * NT);  // floats a warp hands over
   static constexpr int kBytes = kMerge + kWarps * kMergeWarp * 4 + 1024;  // the ring 1024-byte aligned
 };
 struct alignas(16) Meta {
@@ -204,6 +209,12 @@ __device__ __forceinline__ void write_fragment(uint16_t *out, int nh, int lane, 
 // part begins its block's range (slot 0).
 __device__ __forceinline__ size_t part_slot(int first, int first_slot, int i) {
   return (size_t)(first + i) * 2 + (i ? 0 : first_slot);
+}
+
+// Factor that takes what is relative to the maximum `from` to `to`. A side without a
+// visible key holds zeros (or NaN, which stays).
+__device__ __forceinline__ float rescale(float from, float to) {
+  return from == -INFINITY ? 1.0f : ex2_approx(from - to);
 }
 
 // Joins the n parts a, a + step, ... of an item into the output rows, or (out
@@ -566,10 +577,10 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       mult[nt][0] = __shfl_sync(0xffffffffu, inv, t * 8) * p.scale_log2;
       mult[nt][1] = __shfl_sync(0xffffffffu, inv, t * 8 + 4) * p.scale_log2;
     }
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+    float o[NT][D / 16][4], m[NT][2], peak[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = peak[nt][0] = peak[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
@@ -652,29 +663,34 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
         lv[h] = vs[h] > 0.0f ? fmaxf(lg2_approx(vs[h]), -110.0f) : -110.0f;
         lvp[h] = vs[h] > 0.0f ? lv[h] : -INFINITY;
       }
-      float top[NT][2];
+      float top[NT][2], high[NT][2];
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          top[nt][x] = fmaxf(fmaxf(s[0][nt][x], s[0][nt][2 + x]) + lv[0],
-                             fmaxf(s[1][nt][x], s[1][nt][2 + x]) + lv[1]);
-          grow |= top[nt][x] > m[nt][x] + kLazy;
+          const float a = fmaxf(s[0][nt][x], s[0][nt][2 + x]), b = fmaxf(s[1][nt][x], s[1][nt][2 + x]);
+          top[nt][x] = fmaxf(a + lv[0], b + lv[1]);
+          high[nt][x] = fmaxf(a, b);
+          grow |= top[nt][x] > m[nt][x] + kLazy || high[nt][x] > peak[nt][x] + kLazy;
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float mx = top[nt][x];
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            float mx = top[nt][x], pk = high[nt][x];
+#pragma unroll
+            for (int lanes = 4; lanes < 32; lanes *= 2) {
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, lanes));
+              pk = fmaxf(pk, __shfl_xor_sync(0xffffffffu, pk, lanes));
+            }
             mx = fmaxf(mx, m[nt][x]);
-            const float alpha = mx == -INFINITY ? 1.0f : ex2_approx(m[nt][x] - mx);
+            pk = fmaxf(pk, peak[nt][x]);
+            const float alpha = rescale(m[nt][x], mx);
+            l[nt][x] *= rescale(peak[nt][x], pk);
             m[nt][x] = mx;
-            l[nt][x] *= alpha;
+            peak[nt][x] = pk;
 #pragma unroll
             for (int i2 = 0; i2 < D / 16; ++i2) {
               o[nt][i2][x] *= alpha;
@@ -687,13 +703,15 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       for (int nt = 0; nt < NT; ++nt) {
         const float mm[2] = {m[nt][0] == -INFINITY ? 0.0f : m[nt][0],
                              m[nt][1] == -INFINITY ? 0.0f : m[nt][1]};
+        const float pp[2] = {peak[nt][0] == -INFINITY ? 0.0f : peak[nt][0],
+                             peak[nt][1] == -INFINITY ? 0.0f : peak[nt][1]};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float w[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             w[x] = ex2_approx(s[h][nt][x] + (lvp[h] - mm[x & 1]));
-            l[nt][x & 1] += ex2_approx(s[h][nt][x] - mm[x & 1]);
+            l[nt][x & 1] += ex2_approx(s[h][nt][x] - pp[x & 1]);
           }
           pb[h][nt][0] = transpose8x8(pack_half2(w[0], w[1]));
           pb[h][nt][1] = transpose8x8(pack_half2(w[2], w[3]));
@@ -752,7 +770,10 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     }
 
     // ---- the warps' results joined, through shared memory: each warp takes a
-    // quarter of the fragments, from the same lanes of all warps in order.
+    // quarter of the fragments, from the same lanes of all warps in order. The
+    // joint reference of products and sums is the largest score, so that the sum
+    // is at least 2^-8, or 2^48 above it where the values are large: sums of up to
+    // 2^31 keys times 2^8 then leave the products (output times sum) within fp32.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -763,12 +784,16 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       }
     constexpr int kFrags = D / 16 * NT;  // float4 of O per thread
     float4 *const mine = reinterpret_cast<float4 *>(merge + warp * S::kMergeWarp) + lane;
+    auto peaks_of = [&](int w) {  // behind the warp's fragments, maxima and sums
+      return reinterpret_cast<float2 *>(merge + w * S::kMergeWarp + (kFrags + NT) * 32 * 4) + lane;
+    };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
         mine[(nt * (D / 16) + i) * 32] = make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
       mine[(kFrags + nt) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
+      peaks_of(warp)[nt * 32] = make_float2(peak[nt][0], peak[nt][1]);
     }
     __syncthreads();
     {
@@ -777,20 +802,27 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
       const float4 *const from = reinterpret_cast<const float4 *>(merge) + lane;
       constexpr int kStep = S::kMergeWarp / 4;
       float4 ml[kWarps];
-      float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, f[kWarps][2];
+      float2 pk[kWarps];
+      float mx[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY};
+      float sum[2] = {0.0f, 0.0f}, f[kWarps][2];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         ml[w] = from[w * kStep + (kFrags + nt) * 32];
+        pk[w] = peaks_of(w)[nt * 32];
         mx[0] = fmaxf(mx[0], ml[w].x);
         mx[1] = fmaxf(mx[1], ml[w].y);
+        ref[0] = fmaxf(ref[0], pk[w].x);
+        ref[1] = fmaxf(ref[1], pk[w].y);
       }
 #pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (mx[x] - ref[x] > 60.0f) ref[x] += 48.0f;
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        // A side without a visible key holds zeros (or NaN, which stays).
-        f[w][0] = ml[w].x == -INFINITY ? 1.0f : ex2_approx(ml[w].x - mx[0]);
-        f[w][1] = ml[w].y == -INFINITY ? 1.0f : ex2_approx(ml[w].y - mx[1]);
-        sum[0] += ml[w].z * f[w][0];
-        sum[1] += ml[w].w * f[w][1];
+        f[w][0] = rescale(ml[w].x, ref[0]);
+        f[w][1] = rescale(ml[w].y, ref[1]);
+        sum[0] += ml[w].z * rescale(pk[w].x, ref[0]);
+        sum[1] += ml[w].w * rescale(pk[w].y, ref[1]);
       }
       float4 *const my_slot =
           reinterpret_cast<float4 *>(p.slots + ((size_t)blockIdx.x * 2 + slot_of_mine) * kSlotFloats);
@@ -811,11 +843,11 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
         else
           __stcg(my_slot + at * 32 + lane, v);
       }
-      // The maxima and sums of a slot: [column] pairs behind its fragments.
+      // The references and sums of a slot: [column] pairs behind its fragments.
       if (!whole && r == 0 && warp * kShare % (D / 16) == 0) {
         float2 *to = reinterpret_cast<float2 *>(my_slot + kFrags * 32) + nt * 8 + 2 * t;
-        __stcg(to, make_float2(mx[0], sum[0]));
-        __stcg(to + 1, make_float2(mx[1], sum[1]));
+        __stcg(to, make_float2(ref[0], sum[0]));
+        __stcg(to + 1, make_float2(ref[1], sum[1]));
       }
     }
     __syncthreads();  // the merge buffer is free again, the block's stores come before the arrival
