@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import kv8_plain as plain
-from test_gpu_serving import Cache, _done, _dt, _f64, _ints
+from test_gpu_serving import TYPES, Cache, _done, _dt, _f64, _ints
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,29 @@ def test_attn_lower_scores_keep_their_share(gpu, n, heavy, exp):
     got = _attn_call(gpu, c, q, table, [n], 1.0)
     # The sum's n terms are exact powers of two; the output's rounding and the weights'.
     assert (np.abs(got - want) <= want * (2.0 ** -8 + 2.0 ** -10)).all(), got / want
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e5, 1e6])
+def test_attn_one_token_of_a_large_score(gpu, size, t):
+    """A single key is the output whatever its score is: one weight, which is also the sum."""
+    P, d, H, Hq = 16, 64, 4, 36
+    rng = np.random.default_rng(int(size))
+    for lens in ([1], [1, 1, 1]):
+        B = len(lens)
+        c = Cache(gpu, B, H, P, d)
+        table = rng.permutation(B).astype(np.int32)[:, None]
+        c.k.fill_(0)
+        c.k[:, :, :, 0] = _code(1.0)
+        c.v.copy_(torch.from_numpy(plain.to_e4m3(rng.standard_normal((B, H, P, d)) * 100)))
+        c.vs.copy_(torch.from_numpy(rng.uniform(0.5, 2.0, (B, H)).astype(np.float32)))
+        c.ks.copy_(torch.from_numpy(rng.uniform(0.5, 1.0, (B, H)).astype(np.float32)))
+        q = torch.zeros(B, Hq, d, device="cuda")
+        q[:, :, 0] = torch.from_numpy(rng.uniform(0.5, 1.0, (B, Hq)) * rng.choice([-1, 1], (B, Hq)))
+        got = _attn_call(gpu, c, q.to(t), table, lens, size)
+        v = plain.E4M3[c.v.cpu().numpy()][table[:, 0], :, 0] * c.vs.cpu().double().numpy()[table[:, 0], :, None]
+        want = np.repeat(v, Hq // H, axis=1)
+        # The weight's rounding to fp16, the exponentials and fp32 products, the output's.
+        u = torch.finfo(t).eps / 2
+        assert (np.abs(got - want) <= np.abs(want) * (u + 2.0 ** -11 + 2.0 ** -16) + 2.0 ** -24).all(), \
+            (np.abs(got - want) / np.abs(want).clip(1e-9)).max()

@@ -710,8 +710,11 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
           float w[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            w[x] = ex2_approx(s[h][nt][x] + (lvp[h] - mm[x & 1]));
-            l[nt][x & 1] += ex2_approx(s[h][nt][x] - pp[x & 1]);
+            // One difference for both, so that what the sum of a large score and a
+            // scale is rounded by does not come between them.
+            const float below = s[h][nt][x] - pp[x & 1];
+            w[x] = ex2_approx(below + (pp[x & 1] - mm[x & 1] + lvp[h]));
+            l[nt][x & 1] += ex2_approx(below);
           }
           pb[h][nt][0] = transpose8x8(pack_half2(w[0], w[1]));
           pb[h][nt][1] = transpose8x8(pack_half2(w[2], w[3]));
