@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import kv8_plain as plain
-from test_gpu_serving import TYPES, Cache, _done, _dt, _f64, _ints
+from test_gpu_serving import TYPES, Cache, _done, _dt, _f64, _fill, _ints
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,20 @@ def test_attn_one_token_of_a_large_score(gpu, size, t):
         u = torch.finfo(t).eps / 2
         assert (np.abs(got - want) <= np.abs(want) * (u + 2.0 ** -11 + 2.0 ** -16) + 2.0 ** -24).all(), \
             (np.abs(got - want) / np.abs(want).clip(1e-9)).max()
+
+
+def test_attn_zero_scores_of_large_factors(gpu):
+    """Queries and K scales whose product is past fp32's range, at scores that are zero: the largest
+    elements of one meet zeros of the other."""
+    P, d, n = 16, 64, 100
+    rng = np.random.default_rng(3)
+    c, table = _fill(gpu, [n], 1, P, d, rng)
+    q = torch.zeros(1, 4, d, device="cuda").bfloat16()
+    q[:, :, 0] = 2.0 ** 100
+    c.k[:, :, :, 0] = 0
+    c.ks.fill_(2.0 ** 90)
+    got = _attn_call(gpu, c, q, table, [n], 0.2)
+    v = plain.E4M3[c.v.cpu().numpy()] * c.vs.cpu().double().numpy()[:, :, None, None]
+    want = v[table[0]].transpose(0, 2, 1, 3).reshape(-1, d)[:n].mean(0)
+    tol = 2.0 ** -8 * np.abs(want) + np.abs(v[np.isfinite(v)]).max() * (2.0 ** -10 + 2.0 ** -20)
+    assert (np.abs(got - want) <= tol).all()

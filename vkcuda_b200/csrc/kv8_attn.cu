@@ -70,6 +70,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 2;
 constexpr int kMaxHeads = 16;  // query heads of an item
 constexpr float kLazy = 8.0f;  // log2 units
+constexpr float kLargest = 3.402823466e38f;  // of fp32
 
 // Workspace: partial results, two per block (the item that its range starts
 // in and the one that it ends in), then the counters, at offsets that depend
@@ -639,13 +640,18 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
           }
         }
       }
-      // Scores in log2 units; hidden keys -inf.
+      // Scores in log2 units; hidden keys -inf. A factor past fp32's range meets
+      // products that are zero (scores are finite), which stay zero.
+      auto factor = [](float back, float scale) {
+        const float f = back * scale;
+        return f > kLargest ? kLargest : f;
+      };
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[h][nt][x] *= mult[nt][x & 1] * ks[h];
+          for (int x = 0; x < 4; ++x) s[h][nt][x] *= factor(mult[nt][x & 1], ks[h]);
       if (mask != 0xffffffffu) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
