@@ -1,0 +1,50 @@
+"""The serving entries at the ends of their ranges, on the CPU."""
+from __future__ import annotations
+
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+INVALID = 1
+BUF = np.zeros(1 << 12, np.uint8)
+A = (BUF.ctypes.data + 255) & ~255
+
+
+def test_index_arithmetic_at_its_ends(tmp_path):
+    exe = tmp_path / "kv8_ranges"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-I" + os.path.join(ROOT, "vkcuda_b200", "csrc"),
+                    os.path.join(ROOT, "tests", "hosts", "kv8_ranges_host.cpp"), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "PASS\n"
+
+
+@pytest.mark.parametrize("kw", [
+    # Spans that wrap around 64 bits, to a few bytes.
+    dict(Nq=1 << 26, q_strides=[1 << 37, 1 << 37, 1 << 37]),
+    dict(Nk=(1 << 26) + 1, k_strides=[1 << 37, 1 << 37, 1 << 37]),
+    dict(B=2, Nk=(1 << 26) + 1, v_strides=[1 << 37, 1 << 37, 1 << 37]),
+    dict(Nq=(1 << 27) + 1, o_strides=[1 << 37, 1 << 37, 1 << 36])])
+def test_window_spans_past_64_bits(vc, kw):
+    a = dict(Q=A, K=A, V=A, O=A, B=1, Hq=4, Hkv=2, Nq=16, Nk=16, d=64, scale_log2=0.1, dtype=vc.Dtype.F16)
+    a.update(kw)
+    assert vc.flash_window_fwd(**a) == INVALID
+
+
+@pytest.mark.parametrize("kw", [dict(num_pages=(1 << 25) + 1, page_stride=1 << 39),
+                                dict(num_pages=(1 << 30) + 1, scale_stride=1 << 32),
+                                dict(num_pages=(1 << 24) + 1, scale_stride=1 << 38)])
+def test_cache_spans_past_64_bits(vc, kw):
+    c = vc.kv8_cache(**dict(dict(k=A, v=A, k_scale=A, v_scale=A, num_pages=4, heads=2, page_size=16,
+                                 head_dim=64), **kw))
+    assert vc.kv8_append(c, A, A, 2, A, 4, A, 2, 1, vc.Dtype.F16) == INVALID
+    assert vc.kv8_attn(c, A, A, A, 4, A, 1, 4, 0.1, vc.Dtype.F16, A, 1 << 30) == INVALID
+    assert vc.kv8_copy_pages(vc.kv8_layers([c]), A, A, 1) == INVALID
+
+
+def test_append_rows_past_64_bits(vc):
+    c = vc.kv8_cache(A, A, A, A, 4, 2, 16, 64)
+    for kw in (dict(k_stride=1 << 38), dict(v_stride=1 << 37)):
+        assert vc.kv8_append(c, A, A, (1 << 26) + 1, A, 4, A, 1, 1, vc.Dtype.F16, **kw) == INVALID

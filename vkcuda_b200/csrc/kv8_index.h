@@ -50,6 +50,15 @@ VCB_HD int tile_key(const VisibleTiles &t, int i, int tile) {
   return (i < t.head ? i : t.first + (i - t.head)) * tile;
 }
 
+// Entries from the first of `n` rows to the end of the last, which takes `last`:
+// rows lie `stride` >= 0 apart. What is longer than any memory counts as
+// kNoMemory, in sums over several axes too.
+constexpr int64_t kNoMemory = (int64_t)1 << 60;
+VCB_HD int64_t row_span(int64_t n, int64_t stride, int64_t last) {
+  if (n > 1 && stride > (kNoMemory - last) / (n - 1)) return kNoMemory;
+  return n > 1 ? (n - 1) * stride + last : last;
+}
+
 // Split of `total` > 0 tiles over at most `most` blocks, as even as it gets:
 // block c takes [start(c), start(c + 1)), the first `more` blocks one tile more.
 struct TileSplit {

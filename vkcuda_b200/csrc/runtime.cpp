@@ -47,6 +47,7 @@
 #include "../../include/vc/Runtime/VCRuntime.h"
 #include "../../include/vc_b200.h"
 #include "internal.h"
+#include "kv8_index.h"
 
 namespace vc {
 
@@ -1508,10 +1509,17 @@ VCError ints_checked(const void *p, size_t n, const char *name) {
 // A score's factor: positive and finite (a maximum of the products is one of the scores).
 bool positive(float scale) { return scale > 0.0f && scale < INFINITY; }
 
-// Bytes that [B][H][N][d] 16-bit elements at these strides span.
-size_t span16(int B, int H, int N, int d, const int64_t *s) {
-  return (size_t)((B - 1) * s[0] + (H - 1) * s[1] + (int64_t)(N - 1) * s[2] + d) * 2;
+// Whether `entries` of `size` bytes fit behind p. What no memory holds is
+// refused as an argument.
+VCError fits(int64_t entries, size_t size, const void *p, const char *name) {
+  if (entries >= vcb::kNoMemory) return VCError::InvalidValue;
+  return (size_t)entries * size > bytes_available(p) ? too_small(name) : VCError::Success;
 }
+// Entries that [B][H][N][d] at these strides span.
+int64_t span_of(int B, int H, int N, int d, const int64_t *s) {
+  return vcb::row_span(B, s[0], vcb::row_span(H, s[1], vcb::row_span(N, s[2], d)));
+}
+size_t span16(int B, int H, int N, int d, const int64_t *s) { return (size_t)span_of(B, H, N, d, s) * 2; }
 
 VCError flash_window_checked(vcb::FlashWindowArgs f, const int64_t *const strides[4],
                              cudaStream_t s) {
@@ -1535,7 +1543,8 @@ VCError flash_window_checked(vcb::FlashWindowArgs f, const int64_t *const stride
       if (to[i][j] < f.d || to[i][j] % 8 || to[i][j] >= (int64_t)1 << 38) return VCError::InvalidValue;
     }
     if (!p[i] || !aligned(p[i], 16)) return VCError::InvalidValue;
-    if (span16(f.B, H, N, f.d, to[i]) > bytes_available(p[i])) return too_small(name);
+    const VCError e = fits(span_of(f.B, H, N, f.d, to[i]), 2, p[i], name);
+    if (e != VCError::Success) return e;
   }
   VCError e = f.lens ? ints_checked(f.lens, f.B, name) : VCError::Success;
   if (e == VCError::Success) e = ready_to_launch(name, {f.Q, f.K, f.V, f.O, f.lens});
@@ -1564,9 +1573,9 @@ VCError kv8_cache_checked(const vc_kv8_cache &c, const char *name) {
   const void *const p[4] = {c.k, c.v, c.k_scale, c.v_scale};
   for (int i = 0; i < 4; ++i) {
     if (!p[i] || !aligned(p[i], i < 2 ? 16 : 4)) return VCError::InvalidValue;
-    const size_t need = i < 2 ? (size_t)(c.num_pages - 1) * c.page_stride + page
-                              : ((size_t)(c.num_pages - 1) * c.scale_stride + c.heads) * 4;
-    if (need > bytes_available(p[i])) return too_small(name);
+    const VCError e = i < 2 ? fits(vcb::row_span(c.num_pages, c.page_stride, page), 1, p[i], name)
+                            : fits(vcb::row_span(c.num_pages, c.scale_stride, c.heads), 4, p[i], name);
+    if (e != VCError::Success) return e;
   }
   return VCError::Success;
 }
@@ -1576,8 +1585,7 @@ VCError rows_checked(const void *p, int64_t rows, int64_t width, int64_t stride,
     return VCError::InvalidValue;
   if (rows <= 0) return VCError::Success;  // an empty tensor may be null
   if (!p) return VCError::InvalidValue;
-  return (size_t)((rows - 1) * stride + width) * 2 > bytes_available(p) ? too_small(name)
-                                                                        : VCError::Success;
+  return fits(vcb::row_span(rows, stride, width), 2, p, name);
 }
 
 VCError kv8_append_checked(const vcb::Kv8AppendArgs &a, cudaStream_t s) {
