@@ -1,7 +1,8 @@
 // Checks of csrc/kv8_index.h at the ends of its ranges, on the CPU: spans that
-// pass 64 bits.
+// pass 64 bits, the longest sequences with the longest windows and sinks.
 #include <cstdio>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "kv8_index.h"
 
@@ -29,8 +30,31 @@ static void spans() {
   CHECK(row_span(2, (int64_t)1 << 39, row_span((1 << 25) + 1, (int64_t)1 << 39, 1)) == kNoMemory);
 }
 
+// The tiles of a sequence, by their borders: within it, each once, and the
+// visible keys at the borders of the sinks and the window in one of them.
+static void tiles(int len, int window, int sinks, int tile) {
+  const VisibleKeys v = visible_keys(len, window, sinks);
+  const VisibleTiles t = visible_tiles(v, tile);
+  const int64_t end = ((int64_t)len + tile - 1) / tile;
+  CHECK(t.head >= 0 && t.head <= t.first && t.first < end && t.count == t.head + (end - t.first));
+  auto has = [&](int key) { return key / tile < t.head || key / tile >= t.first; };
+  for (int key : {0, v.sink - 1, v.sink, v.lo - 1, v.lo, len - 1}) {
+    if (key < 0 || key >= len) continue;
+    const bool see = window <= 0 || key >= (int64_t)len - window || key < sinks;
+    CHECK(key_visible(v, key) == see);
+    if (see) CHECK(has(key));
+  }
+  CHECK(tile_key(t, 0, tile) == (t.head || !t.first ? 0 : t.first * tile));
+  CHECK(tile_key(t, t.count - 1, tile) == (end - 1) * tile);
+}
+
 int main() {
   spans();
+  const int most = 2147483647;
+  for (int len : {1, 100, 128, 129, most - 128, most - 127, most - 15, most - 1, most})
+    for (int window : {0, 1, 64, 128, 1 << 30, most - 1, most})
+      for (int sinks : {0, 1, 128, 1 << 30, most - 127, most - 126, most - 1, most})
+        for (int tile : {16, 64, 128}) tiles(len, window, sinks, tile);
   std::printf("PASS\n");
   return 0;
 }

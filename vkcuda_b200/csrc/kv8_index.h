@@ -40,7 +40,7 @@ VCB_HD VisibleTiles visible_tiles(const VisibleKeys &v, int tile) {
   VisibleTiles t;
   t.first = v.lo / tile;
   const int end = (int)(((int64_t)v.len + tile - 1) / tile);
-  t.head = (v.sink + tile - 1) / tile;
+  t.head = (int)(((int64_t)v.sink + tile - 1) / tile);
   if (t.head > t.first) t.head = t.first;  // the window's first tile holds the rest
   t.count = t.head + end - t.first;
   return t;
