@@ -48,3 +48,14 @@ def test_append_rows_past_64_bits(vc):
     c = vc.kv8_cache(A, A, A, A, 4, 2, 16, 64)
     for kw in (dict(k_stride=1 << 38), dict(v_stride=1 << 37)):
         assert vc.kv8_append(c, A, A, (1 << 26) + 1, A, 4, A, 1, 1, vc.Dtype.F16, **kw) == INVALID
+
+
+def test_window_waits_cover_the_longest_pair(tmp_path):
+    """A wait that lasts as long as a pair of row tiles grows with its keys: 4 s alone were too short
+    from 2^28 keys on."""
+    from vkcuda_b200 import build
+    exe = tmp_path / "window_wait"
+    cuda = os.path.join(os.path.dirname(os.path.dirname(build.nvcc())), "include")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-I" + cuda, "-I" + os.path.join(ROOT, "vkcuda_b200", "csrc"),
+                    os.path.join(ROOT, "tests", "hosts", "window_wait_host.cpp"), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "PASS\n"

@@ -139,6 +139,7 @@ struct WindowParams {
   int Hq, Hkv, Nq, Nk, window, sinks;
   int items, slices;  // pairs (split: row tiles) of a slice (a sequence's K/V head); slices
   float scale_log2;
+  uint64_t pair_wait_ns;  // limit of the waits that a whole pair may take
 };
 
 // Order of the grid: groups of K/V slices, the last rows (with the most keys)
@@ -494,7 +495,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         int stage = 0, n_live = 0, n_clean = 0;
         bool live = false;  // the last pair had keys
         for (int r = 0;; ++r) {
-          if (!mbar_wait_idle(&bars->work_empty[r & 1], ((r >> 1) & 1) ^ 1)) break;
+          if (!mbar_wait_idle(&bars->work_empty[r & 1], ((r >> 1) & 1) ^ 1, p.pair_wait_ns)) break;
           Work &k = bars->work[r & 1];
           bool have = true;
           if (r > 0) {
@@ -592,7 +593,8 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     } else if (warp == 11) {
       // ------------------------------------------------ V behind a sequence's end
       auto idle_work = [&]() {
-        return __all_sync(0xffffffffu, mbar_wait_idle(&bars->work_full[round & 1], (round >> 1) & 1)) &&
+        return __all_sync(0xffffffffu, mbar_wait_idle(&bars->work_full[round & 1], (round >> 1) & 1,
+                                                      p.pair_wait_ns)) &&
                bars->work[round & 1].valid;
       };
       for (bool ok = true; ok && idle_work(); done()) {
@@ -601,7 +603,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
         // The issuer has seen the stage arrive; it stays until the issuer goes on
         // (a stage's own barrier may be phases behind when this warp comes here).
         const int s = k.stage0 + k.total + SPLIT, st = s % kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_dirty, k.n_clean & 1) &&
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_dirty, k.n_clean & 1, p.pair_wait_ns) &&
                                          mbar_wait(&bars->kv_full[st], (s / kStages) & 1));
         if (!ok) break;
         // 128-byte rows of tokens in each box.
@@ -810,6 +812,7 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   p.window = a.window;
   p.sinks = a.sinks;
   p.scale_log2 = a.scale_log2;
+  p.pair_wait_ns = window_pair_wait_ns(a.Nk);
   const int64_t units = ((int64_t)a.Nq + BQ - 1) / BQ * (a.Hq / a.Hkv);
   if (units * a.B * a.Hkv > INT32_MAX / kOrderGroup) return cudaErrorInvalidValue;
   p.slices = a.B * a.Hkv;

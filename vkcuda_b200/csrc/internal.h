@@ -119,6 +119,10 @@ struct FlashWindowArgs {
   int dtype;
 };
 cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream);
+// Limit of the waits in flash_window.cu that last as long as a pair of row tiles
+// does: 16 us for each of its 128-key steps, which take 2, beside the 4 s that
+// every wait has.
+constexpr uint64_t window_pair_wait_ns(int Nk) { return 4000000000ull + ((uint64_t)Nk / 128 + 1) * 16000; }
 
 // ---- 8-bit paged K/V cache (kv8_pages.cu, kv8_attn.cu)
 struct Kv8AppendArgs {
