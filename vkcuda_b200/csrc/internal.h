@@ -157,15 +157,23 @@ struct Kv8AttnArgs {
 size_t kv8_attn_workspace_bytes(const vc_kv8_cache &c, int B, int Hq);
 cudaError_t launch_kv8_attn(const Kv8AttnArgs &a, cudaStream_t stream);
 
-// ---- device error words, one accessor per translation unit
+// ---- device error words, two accessors per translation unit
 int stream_kernels_error(int clear);
+void *stream_kernels_error_word();
 int gemm_tcgen05_error(int clear);
+void *gemm_tcgen05_error_word();
 int gemm_f32_error(int clear);
+void *gemm_f32_error_word();
 int flash_tcgen05_error(int clear);
+void *flash_tcgen05_error_word();
 int selftest_error(int clear);
+void *selftest_error_word();
 int flash_window_error(int clear);
+void *flash_window_error_word();
 int kv8_pages_error(int clear);
+void *kv8_pages_error_word();
 int kv8_attn_error(int clear);
+void *kv8_attn_error_word();
 cudaError_t launch_selftest_bounded_wait(unsigned timeout_us, cudaStream_t stream);
 
 // ---- runtime-owned scratch (runtime.cpp): per (device, stream) partials

@@ -739,7 +739,8 @@ __device__ __forceinline__ float ex2_approx(float x) {
 
 }  // namespace vcb
 
-// Host accessor for this unit's error word: returns it, clears it when asked.
+// Host accessors for this unit's error word: one returns it, and clears it when
+// asked; one its address on the current device, or null.
 #define VCB_DEFINE_ERROR_ACCESSOR(fname)                                  \
   namespace vcb {                                                         \
   int fname(int clear) {                                                  \
@@ -751,5 +752,10 @@ __device__ __forceinline__ float ex2_approx(float x) {
       cudaMemcpyToSymbol(vc_dev_error, &z, sizeof(z));                    \
     }                                                                     \
     return static_cast<int>(v);                                           \
+  }                                                                       \
+  void *fname##_word() {                                                  \
+    void *at = nullptr;                                                   \
+    return cudaGetSymbolAddress(&at, vc_dev_error) == cudaSuccess ? at    \
+                                                                  : nullptr; \
   }                                                                       \
   }

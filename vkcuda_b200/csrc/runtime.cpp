@@ -2259,13 +2259,30 @@ int vc_kernel_set_constant(void *k, const char *name, long long value) {
 int vc_kernel_error(int clear) {
   if (!ensure_init()) return E(VCError::InitializationError);
   use_current_device();
-  int codes[8] = {vcb::stream_kernels_error(clear), vcb::gemm_tcgen05_error(clear),
-                  vcb::gemm_f32_error(clear), vcb::flash_tcgen05_error(clear),
-                  vcb::selftest_error(clear), vcb::flash_window_error(clear),
-                  vcb::kv8_pages_error(clear), vcb::kv8_attn_error(clear)};
-  for (int c : codes)
-    if (c != 0) return c;
-  return 0;
+  // All units' words come with one wait (a synchronous copy each: 12 us a unit).
+  constexpr int kUnits = 8;
+  void *const at[kUnits] = {vcb::stream_kernels_error_word(), vcb::gemm_tcgen05_error_word(),
+                            vcb::gemm_f32_error_word(),       vcb::flash_tcgen05_error_word(),
+                            vcb::selftest_error_word(),       vcb::flash_window_error_word(),
+                            vcb::kv8_pages_error_word(),      vcb::kv8_attn_error_word()};
+  static std::mutex mu;
+  static unsigned *words = nullptr;  // pinned, kept
+  std::lock_guard<std::mutex> lk(mu);
+  if (!words && cudaHostAlloc(reinterpret_cast<void **>(&words), kUnits * sizeof(unsigned),
+                              cudaHostAllocPortable) != cudaSuccess)
+    return -1;
+  for (int i = 0; i < kUnits; ++i)
+    if (!at[i] || cudaMemcpyAsync(&words[i], at[i], sizeof(unsigned), cudaMemcpyDeviceToHost, nullptr) != cudaSuccess)
+      return -1;
+  if (cudaStreamSynchronize(nullptr) != cudaSuccess) return -1;
+  int code = 0;
+  for (int i = 0; i < kUnits; ++i) {
+    if (!words[i]) continue;
+    if (code == 0) code = static_cast<int>(words[i]);
+    if (clear) cudaMemsetAsync(at[i], 0, sizeof(unsigned), nullptr);
+  }
+  if (clear && code) cudaStreamSynchronize(nullptr);
+  return code;
 }
 int vc_selftest_bounds_check(void) {
   if (!ensure_init()) return -1;
