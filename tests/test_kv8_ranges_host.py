@@ -59,3 +59,24 @@ def test_window_waits_cover_the_longest_pair(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-Wall", "-I" + cuda, "-I" + os.path.join(ROOT, "vkcuda_b200", "csrc"),
                     os.path.join(ROOT, "tests", "hosts", "window_wait_host.cpp"), "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "PASS\n"
+
+
+def test_addresses_without_exceptions(vc):
+    """Host arrays and ctypes objects, which most calls of the runtime get, reach their address by
+    tests, not by a caught exception (0.15 instead of 0.65 us)."""
+    import ctypes
+    import sys
+    array, words, raw = np.zeros(3), (ctypes.c_int * 3)(), bytearray(8)
+    raised = []
+    mon = sys.monitoring
+    mon.use_tool_id(mon.PROFILER_ID, "addresses")
+    mon.register_callback(mon.PROFILER_ID, mon.events.RAISE, lambda *a: raised.append(a))
+    mon.set_events(mon.PROFILER_ID, mon.events.RAISE)
+    try:
+        got = [vc._addr(x) for x in (array, words, raw, 5, None)]
+    finally:
+        mon.set_events(mon.PROFILER_ID, 0)
+        mon.free_tool_id(mon.PROFILER_ID)
+    assert got[:2] == [array.ctypes.data, ctypes.addressof(words)] and got[3:] == [5, None]
+    assert not raised
+    assert [vc._at(x) for x in (array, words, 5, None)] == got[:2] + got[3:]

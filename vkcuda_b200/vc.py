@@ -190,14 +190,12 @@ def library() -> ctypes.CDLL:
 
 def _addr(x) -> Optional[int]:
     """Address of a host or device buffer (int, numpy array, ctypes object, torch tensor)."""
-    if x is None or type(x) is int:
-        return x
-    try:  # a tensor, as the serving calls mostly get
-        return x.data_ptr()
-    except AttributeError:
-        pass
+    if x is None:
+        return None
     if isinstance(x, int):
-        return int(x)
+        return x
+    if hasattr(x, "data_ptr"):
+        return x.data_ptr()
     if hasattr(x, "__array_interface__"):
         return x.__array_interface__["data"][0]
     if isinstance(x, (bytearray, memoryview)):
@@ -590,6 +588,16 @@ _ERRORS = tuple(VCError)        # by value: their construction is a tenth of a s
 _Strides = ctypes.c_int64 * 3
 
 
+def _at(x) -> Optional[int]:
+    """As _addr, for arguments that are tensors as a rule (0.1 us instead of 0.17)."""
+    if x is None or type(x) is int:
+        return x
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return _addr(x)
+
+
 def _strides(s):
     """Three element strides (batch, head, token), or None for a dense [B][H][N][d]."""
     return None if s is None else _Strides(*s)
@@ -602,8 +610,8 @@ def flash_window_fwd(Q, K, V, O, B: int, Hq: int, Hkv: int, Nq: int, Nk: int, d:
     """Causal attention of prompts through a sliding window with sinks, K/V heads
     shared by groups of query heads (vc_flash_window_fwd)."""
     return _ERRORS[library().vc_flash_window_fwd(
-        _addr(Q), _addr(K), _addr(V), _addr(O), B, Hq, Hkv, Nq, Nk, d, _strides(q_strides),
-        _strides(k_strides), _strides(v_strides), _strides(o_strides), _addr(lens), window, sinks,
+        _at(Q), _at(K), _at(V), _at(O), B, Hq, Hkv, Nq, Nk, d, _strides(q_strides),
+        _strides(k_strides), _strides(v_strides), _strides(o_strides), _at(lens), window, sinks,
         float(scale_log2), int(dtype), _stream(stream))]
 
 
@@ -619,7 +627,7 @@ class Kv8Cache(ctypes.Structure):
 def kv8_cache(k, v, k_scale, v_scale, num_pages: int, heads: int, page_size: int, head_dim: int,
               page_stride: int = 0, scale_stride: int = 0) -> Kv8Cache:
     """A layer's cache over device buffers that the caller keeps; strides 0: dense."""
-    return Kv8Cache(_addr(k), _addr(v), _addr(k_scale), _addr(v_scale), num_pages, heads, page_size,
+    return Kv8Cache(_at(k), _at(v), _at(k_scale), _at(v_scale), num_pages, heads, page_size,
                     head_dim, page_stride or heads * page_size * head_dim, scale_stride or heads)
 
 
@@ -634,8 +642,8 @@ def kv8_append(cache: Kv8Cache, K, V, tokens: int, table, table_width: int, star
     """Quantise new K/V tokens into their sequences' pages (vc_kv8_append); strides 0: dense."""
     row = cache.heads * cache.head_dim
     return _ERRORS[library().vc_kv8_append(
-        ctypes.byref(cache), _addr(K), _addr(V), k_stride or row, v_stride or row, tokens,
-        _addr(table), table_width, _addr(start), _addr(cu), B, max_new, _addr(lens_out), int(dtype),
+        ctypes.byref(cache), _at(K), _at(V), k_stride or row, v_stride or row, tokens,
+        _at(table), table_width, _at(start), _at(cu), B, max_new, _at(lens_out), int(dtype),
         _stream(stream))]
 
 
@@ -652,14 +660,14 @@ def kv8_attn(cache: Kv8Cache, Q, O, table, table_width: int, lens, B: int, Hq: i
     """Attention of one token for each sequence over the cache (vc_kv8_attn); strides 0: dense."""
     row = Hq * cache.head_dim
     return _ERRORS[library().vc_kv8_attn(
-        ctypes.byref(cache), _addr(Q), q_stride or row, _addr(O), o_stride or row, _addr(table),
-        table_width, _addr(lens), B, Hq, window, sinks, float(scale_log2), int(dtype),
-        _addr(workspace), workspace_bytes, _stream(stream))]
+        ctypes.byref(cache), _at(Q), q_stride or row, _at(O), o_stride or row, _at(table),
+        table_width, _at(lens), B, Hq, window, sinks, float(scale_log2), int(dtype),
+        _at(workspace), workspace_bytes, _stream(stream))]
 
 
 def kv8_copy_pages(layers, src, dst, n: int, stream=None) -> VCError:
     """Copy pages src[i] -> dst[i] in every layer (kv8_layers), codes and scales."""
-    return _ERRORS[library().vc_kv8_copy_pages(layers, len(layers), _addr(src), _addr(dst), n,
+    return _ERRORS[library().vc_kv8_copy_pages(layers, len(layers), _at(src), _at(dst), n,
                                                _stream(stream))]
 
 
