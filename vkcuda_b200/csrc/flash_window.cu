@@ -52,6 +52,7 @@
 #include <cstdint>
 #include <mutex>
 
+#include "dependent_launch.cuh"
 #include "internal.h"
 #include "ptx.cuh"
 
@@ -491,7 +492,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
     if (warp == 10) {
       // ------------------------------------------------ scheduler
       if (lane == 0) {
-        int x = blockIdx.x, y = 0;
+        int x = blockIdx.x;
         int stage = 0, n_live = 0, n_clean = 0;
         bool live = false;  // the last pair had keys
         for (int r = 0;; ++r) {
@@ -502,7 +503,7 @@ flash_window_kernel(const __grid_constant__ WindowParams p) {
             mbar_arrive_expect_tx(&bars->answer_full, 16);
             steal_cta(&bars->answer, &bars->answer_full);
             have = mbar_wait(&bars->answer_full, (r - 1) & 1) &&
-                   stolen_cta(smem_u32(&bars->answer), x, y);
+                   stolen_cta(smem_u32(&bars->answer), x);
             fence_proxy_async_smem();  // read before the queue writes there again
           }
           k.valid = have;
@@ -775,17 +776,8 @@ cudaError_t launch_typed(const WindowParams &p, int grid, cudaStream_t stream) {
       if (dev < 64) configured |= (1ull << dev);
     }
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = WindowSmem<HD>::kBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, flash_window_kernel<HD, BF16, SPLIT>, p);
+  return launch_dependent(flash_window_kernel<HD, BF16, SPLIT>, dim3((unsigned)grid), kThreads,
+                          (int)WindowSmem<HD>::kBytes, p, stream);
 }
 
 template <int HD, bool BF16>

@@ -53,6 +53,7 @@
 #include <cstdint>
 #include <mutex>
 
+#include "dependent_launch.cuh"
 #include "internal.h"
 #include "kv8_index.h"
 #include "ptx.cuh"
@@ -900,24 +901,6 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
   }
 }
 
-// A launch that may begin while the one before it ends (it waits for that
-// one's results itself).
-cudaError_t launch_dependent(const void *kernel, dim3 grid, int threads, int smem,
-                             const AttnParams &p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  void *args[] = {const_cast<AttnParams *>(&p)};
-  return cudaLaunchKernelExC(&cfg, kernel, args);
-}
-
 template <int D, int NT, bool BF16>
 cudaError_t launch_typed(const AttnParams &p, cudaStream_t stream) {
   constexpr int bytes = Smem<D, NT>::kBytes;
@@ -935,8 +918,7 @@ cudaError_t launch_typed(const AttnParams &p, cudaStream_t stream) {
       if (dev < 64) configured |= (1ull << dev);
     }
   }
-  return launch_dependent(reinterpret_cast<const void *>(kv8_attn_kernel<D, NT, BF16>),
-                          dim3(grid_blocks()), kThreads, bytes, p, stream);
+  return launch_dependent(kv8_attn_kernel<D, NT, BF16>, dim3(grid_blocks()), kThreads, bytes, p, stream);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,

@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <mutex>
 
+#include "dependent_launch.cuh"
 #include "internal.h"
 #include "kv8_index.h"
 #include "ptx.cuh"
@@ -219,24 +220,6 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
     for (int i = 0; i < PASSES; ++i) x[i] = next[i];
     old_raw = old_next;
   }
-}
-
-// A launch that may begin while the one before it ends (it waits for that
-// one's results itself).
-template <class P>
-cudaError_t launch_dependent(void (*kernel)(P), dim3 grid, int threads, int smem, const P &p,
-                             cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.dynamicSmemBytes = smem;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 // At most 4 passes: 32 bytes of a token's tile in a thread's registers, and as

@@ -98,8 +98,9 @@ __device__ __forceinline__ bool mbar_test_nb(uint32_t bar_addr, uint32_t parity)
 // Wait for the completion of the barrier phase whose parity is `parity`.
 // Bounded by `limit_ns` of wall time; false (and an error recorded) on
 // timeout. `limit_ns` defaults to 4 s, far above any legitimate wait here.
-__device__ __forceinline__ bool mbar_wait_at(uint32_t addr, uint32_t parity,
-                                             uint64_t limit_ns = 4000000000ull) {
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
+                                          uint64_t limit_ns = 4000000000ull) {
+  const uint32_t addr = smem_u32(bar);
   if (mbar_test_nb(addr, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   for (uint32_t spin = 1;; ++spin) {
@@ -109,11 +110,6 @@ __device__ __forceinline__ bool mbar_wait_at(uint32_t addr, uint32_t parity,
       return false;
     }
   }
-}
-
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
-                                          uint64_t limit_ns = 4000000000ull) {
-  return mbar_wait_at(smem_u32(bar), parity, limit_ns);
 }
 
 // As mbar_wait, for a warp that waits long beside busy ones: it sleeps between
@@ -231,7 +227,7 @@ __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *m
       : "memory");
 }
 
-// 2D / 3D / 4D tiled store shared -> global (bulk async group).
+// 2D / 3D tiled store shared -> global (bulk async group).
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map,
                                              const void *smem_src, int32_t x,
                                              int32_t y) {
@@ -261,15 +257,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map,
       "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
           reinterpret_cast<uint64_t>(map)),
       "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, const void *smem_src,
-                                             int32_t x, int32_t y, int32_t z, int32_t w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
-          reinterpret_cast<uint64_t>(map)),
-      "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
 
@@ -333,21 +320,19 @@ __device__ __forceinline__ void steal_cta(void *smem_dst, uint64_t *bar) {
       "r"(smem_u32(bar))
       : "memory");
 }
-// The stolen CTA's index; false when none was left.
-__device__ __forceinline__ bool stolen_cta(uint32_t smem_addr, int &x, int &y) {
-  uint32_t ok, cx = 0, cy = 0;
+// The stolen CTA's index in a 1-D grid; false when none was left.
+__device__ __forceinline__ bool stolen_cta(uint32_t smem_addr, int &x) {
+  uint32_t ok, cx = 0;
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
-      "ld.shared.b128 r, [%3];\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
       "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %2, r;\n\t}"
-      : "=r"(ok), "=r"(cx), "=r"(cy)
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(ok), "=r"(cx)
       : "r"(smem_addr)
       : "memory");
   x = (int)cx;
-  y = (int)cy;
   return ok != 0;
 }
 
@@ -412,12 +397,12 @@ __device__ __forceinline__ void mma_f16_ts_lohi(uint32_t d_tmem, uint32_t a_tmem
 
 // Arrive (once) on `bar` when every tcgen05.mma issued so far by this thread
 // has completed.
-__device__ __forceinline__ void mma_commit_at(uint32_t bar_addr) {
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr)
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t *bar) { mma_commit_at(smem_u32(bar)); }
 
 // The same, executed by a whole converged warp of which one elected lane issues
 // (operands that every lane computes alike stay warp-uniform).
