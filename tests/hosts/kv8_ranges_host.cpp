@@ -1,5 +1,6 @@
 // Checks of csrc/kv8_index.h at the ends of its ranges, on the CPU: spans that
-// pass 64 bits, the longest sequences with the longest windows and sinks.
+// pass 64 bits, the longest sequences with the longest windows and sinks, and
+// the masks that the kernel takes its keys by.
 #include <cstdio>
 #include <cstdlib>
 #include <initializer_list>
@@ -44,6 +45,17 @@ static void tiles(int len, int window, int sinks, int tile) {
     CHECK(key_visible(v, key) == see);
     if (see) CHECK(has(key));
   }
+  // A warp's 32 keys of a tile, bit by bit, at every tile of short sequences and
+  // around the borders of long ones.
+  auto mask = [&](int64_t tile0) {
+    for (int64_t key = tile0; key < tile0 + 128 && key + 31 <= 2147483647; key += 32)
+      for (int i = 0; i < 32; ++i)
+        CHECK((visible_mask(v, (int)key) >> i & 1) == (uint32_t)key_visible(v, (int)key + i));
+  };
+  if (len <= 1100)
+    for (int64_t k = 0; k < end * tile; k += 128) mask(k);
+  else
+    for (int64_t key : {(int64_t)0, (int64_t)v.sink, (int64_t)v.lo, (int64_t)len - 1}) mask(key / 128 * 128);
   CHECK(tile_key(t, 0, tile) == (t.head || !t.first ? 0 : t.first * tile));
   CHECK(tile_key(t, t.count - 1, tile) == (end - 1) * tile);
 }
@@ -51,6 +63,9 @@ static void tiles(int len, int window, int sinks, int tile) {
 int main() {
   spans();
   const int most = 2147483647;
+  for (int len : {1, 31, 32, 33, 127, 128, 129, 500, 1023, 1100})
+    for (int window : {0, 1, 2, 17, 31, 32, 33, 100, 128, 511, 5000})
+      for (int sinks : {0, 1, 4, 31, 32, 33, 64, 130, 2000}) tiles(len, window, sinks, 128);
   for (int len : {1, 100, 128, 129, most - 128, most - 127, most - 15, most - 1, most})
     for (int window : {0, 1, 64, 128, 1 << 30, most - 1, most})
       for (int sinks : {0, 1, 128, 1 << 30, most - 127, most - 126, most - 1, most})

@@ -179,11 +179,6 @@ struct alignas(16) Meta {
 };
 static_assert(sizeof(Meta) == 32, "two 16-byte words a stage");
 
-// The low n bits.
-__device__ __forceinline__ uint32_t low_bits(int n) {
-  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
-}
-
 // Fragment i of a thread of the O^T product: d = r D / 8 + 2 i and + 1, columns
 // (query heads) 2t and 2t + 1 of nt (x, z: the first column; y, w: the second),
 // divided by the columns' sums into the output rows (of nh heads from `out` on).
@@ -429,9 +424,6 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
   const bool two = p.page_shift == 4;  // pages of 16 tokens: two per step
   Cursor pre = cur;
   int64_t pre_t = t0;
-  auto any_visible = [&](const Cursor &c, int k0, int n) {
-    return k0 < c.vis.len && (k0 + n - 1 >= c.vis.lo || k0 < c.vis.sink);
-  };
   // Pages of the item's tiles from `pages_at` on, one tile per lane, and their
   // scales; a lane issues the copies of its own tile.
   int pages[2] = {-1, -1}, pages_at = 0;
@@ -445,10 +437,11 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
     const int k0 = tile_key(pre.tiles, i, kTile) + warp * 32;
     const int32_t *row = p.table + (int64_t)pre.b * p.table_width;
     const int head = pre.item / p.groups;
+    const uint32_t mask = visible_mask(pre.vis, k0);
     bool bad = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (!any_visible(pre, k0 + 16 * h, 16)) continue;
+      if (!(mask >> 16 * h & 0xffffu)) continue;
       pages[h] = row[(k0 + 16 * h) >> p.page_shift];
       if (pages[h] < 0 || pages[h] >= p.num_pages) {
         pages[h] = -1;
@@ -490,8 +483,7 @@ kv8_attn_kernel(const __grid_constant__ AttnParams p) {
   auto publish = [&](int stage, int tile, uint32_t bytes) {
     if (lane != tile - pages_at) return;
     const int k0 = tile_key(pre.tiles, tile, kTile) + warp * 32;
-    uint32_t mask = low_bits(pre.vis.len - k0) &
-                    (~low_bits(pre.vis.lo - k0) | low_bits(pre.vis.sink - k0));
+    uint32_t mask = visible_mask(pre.vis, k0);
     if (pages[0] < 0) mask &= 0xffff0000u;
     if (pages[1] < 0) mask &= 0x0000ffffu;
     Meta &m = metas[stage];

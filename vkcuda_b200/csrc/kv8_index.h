@@ -30,6 +30,12 @@ VCB_HD VisibleKeys visible_keys(int len, int window, int sinks) {
 VCB_HD bool key_visible(const VisibleKeys &v, int key) {
   return key < v.len && (key >= v.lo || key < v.sink);
 }
+// The low n bits.
+VCB_HD uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
+// The same for the 32 keys from `key` on, one bit each.
+VCB_HD uint32_t visible_mask(const VisibleKeys &v, int key) {
+  return low_bits(v.len - key) & (~low_bits(v.lo - key) | low_bits(v.sink - key));
+}
 
 // Those keys as tiles of `tile` keys aligned to multiples of `tile`: first
 // `head` tiles from key 0 (the sinks), then the window's from tile `first`.
