@@ -1,5 +1,6 @@
-"""The cache attention at the ends of its documented range: value scales, scores
-and lengths, against closed forms and the float64 forms of kv8_plain.py."""
+"""The serving attentions at the ends of their documented ranges: value scales and
+scores, against closed forms and the float64 forms of kv8_plain.py; and the same
+bits from call to call."""
 from __future__ import annotations
 
 import numpy as np
@@ -116,3 +117,31 @@ def test_attn_zero_scores_of_large_factors(gpu):
     want = v[table[0]].transpose(0, 2, 1, 3).reshape(-1, d)[:n].mean(0)
     tol = 2.0 ** -8 * np.abs(want) + np.abs(v[np.isfinite(v)]).max() * (2.0 ** -10 + 2.0 ** -20)
     assert (np.abs(got - want) <= tol).all()
+
+
+WINDOW_REPEATS = [
+    # B, Hq, Hkv, Nq, Nk, d, window, sinks, lens: few row tiles, whose keys are shared, and many
+    (1, 8, 2, 97, 97, 64, 64, 4, None), (1, 8, 1, 2000, 2000, 128, 0, 0, None),
+    (4, 16, 4, 700, 1100, 128, 300, 130, None), (5, 16, 4, 1000, 1000, 128, 256, 4, [1000, 3, 0, 640, 129]),
+    (2, 32, 8, 900, 2000, 64, 0, 0, None),
+]
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("shape", WINDOW_REPEATS)
+def test_window_same_answer_each_time(gpu, shape, t):
+    """Call after call, with and without a wait between, and beside another stream's calls: the same
+    bits, although the row tiles go to whichever CTA asks first."""
+    B, Hq, Hkv, Nq, Nk, d, window, sinks, lens = shape
+    q, k, v = (torch.randn(B, H, N, d, device="cuda").to(t) for H, N in ((Hq, Nq), (Hkv, Nk), (Hkv, Nk)))
+    ln = None if lens is None else _ints(lens)
+    streams = [None, torch.cuda.Stream()]
+    outs = [torch.full_like(q, 7.0) for _ in range(24)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert gpu.flash_window_fwd(q, k, v, o, B, Hq, Hkv, Nq, Nk, d, 0.15, _dt(gpu, t), window=window,
+                                    sinks=sinks, lens=ln, stream=streams[i >= 8 and i % 2]) == 0
+        if i < 4:
+            torch.cuda.synchronize()
+    _done(gpu)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
