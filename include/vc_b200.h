@@ -262,7 +262,14 @@ int vc_flash_fwd(const void *Q, const void *K, const void *V, void *O, int BH,
  * vc_launch_kernel does.
  * What lies in device memory (lengths, offsets, page numbers) is checked by
  * the kernels: what is out of range is left out and vc_kernel_error reports
- * it (4, out of bounds). */
+ * it (4, out of bounds); the lengths of vc_flash_window_fwd are clamped and
+ * not reported.
+ * Refused are sizes beyond 2^30 for Nq and Nk, 65535 for B * Hq of
+ * vc_flash_window_fwd, for B and Hq of vc_kv8_attn and for a cache's heads, 2^30
+ * bytes for a page's codes of one layer's K or V and 2^31 - 1 tokens for
+ * vc_kv8_attn's row of a page table; strides of 2^38 elements (pages: 2^40 bytes)
+ * and more; batches with 2^28 row tiles of 128 rows, or 2^31 pages or tiles of
+ * 128 keys. */
 
 /* Causal flash attention of prompts through a sliding window, with a few first
  * tokens that stay visible (sinks). Query row i of a sequence stands at
@@ -272,9 +279,9 @@ int vc_flash_fwd(const void *Q, const void *K, const void *V, void *O, int BH,
  *   p = softmax_2(scale_log2 * Q[b][h][i] . K[b][h / (Hq / Hkv)][j]).
  * A row that sees no key (t < 0) is zero. scale_log2 is positive, Hq is a multiple of Hkv, d 64 or
  * 128, dtype F16 or BF16. The strides (elements between batches, heads and
- * tokens, in this order; NULL: dense [B][H][N][d]) are multiples of 8, rows
- * contiguous and 16-byte aligned; along an axis of one entry they do not
- * matter. `lens` (optional, device, B entries): sequence b has lens[b] tokens
+ * tokens, in this order; NULL: dense [B][H][N][d]) are multiples of 8 and at
+ * least d, rows contiguous and 16-byte aligned; along an axis of one entry they
+ * do not matter. `lens` (optional, device, B entries): sequence b has lens[b] tokens
  * (clamped to [0, Nk]); what K and V hold behind them is not used, whatever it
  * is, and rows of O at positions t >= lens[b] are left as they were. V of a
  * sequence's own tokens has to be finite, as for vc_flash_fwd. */
@@ -322,13 +329,15 @@ int vc_kv8_append(const vc_kv8_cache *cache, const void *K, const void *V, int64
  * at position lens[b] - 1, and sees the keys j < lens[b] with
  * j >= lens[b] - window (window 0: all) or j < sinks. lens[b] = 0 gives a zero
  * row. scale_log2 is positive, Hq a multiple of cache->heads. Any positive scales within 2^-100 ..
- * 2^119 (and 0) are taken. Several tokens of one sequence (a draft to verify)
+ * 2^119 (and 0) are taken. Weights times value scales have fp16's range below
+ * their largest: what is less than 2^-25 of it counts in the sum alone.
+ * Several tokens of one sequence (a draft to verify)
  * are several rows with the same pages and growing lens.
  * workspace: vc_kv8_attn_workspace bytes, 256-byte aligned, zero before its
  * first call and left ready for the next, of whatever shape; calls that may
  * overlap (two streams, two graphs) need one each, and after a kernel error 1
  * (a wait that ran out) it is zeroed again. The scores have to be finite in
- * fp32; batch and table sizes with 2^31 or more tiles of 128 keys are refused. */
+ * fp32. */
 int vc_kv8_attn_workspace(const vc_kv8_cache *cache, int B, int Hq, size_t *bytes);
 int vc_kv8_attn(const vc_kv8_cache *cache, const void *Q, int64_t q_stride, void *O,
                 int64_t o_stride, const int32_t *table, int table_width, const int32_t *lens,
@@ -348,7 +357,8 @@ int vc_kv8_copy_pages(const vc_kv8_cache *layers, int n_layers, const int32_t *s
 int vc_kv8_pool_create(void **pool, int num_pages, int page_size);
 int vc_kv8_pool_destroy(void *pool);
 int vc_kv8_pool_new(void *pool, int64_t *seq);  /* an empty sequence */
-/* A sequence with the same tokens, on the same pages. */
+/* A sequence with the same tokens, on the same pages. Sequences only grow: a
+ * draft that may be rejected goes into a fork, which is freed then. */
 int vc_kv8_pool_fork(void *pool, int64_t seq, int64_t *child);
 /* Room for `tokens` more: VC_OUT_OF_MEMORY when the free pages do not hold
  * them. When the first of them falls into a page that another sequence holds

@@ -80,3 +80,31 @@ def test_addresses_without_exceptions(vc):
     assert got[:2] == [array.ctypes.data, ctypes.addressof(words)] and got[3:] == [5, None]
     assert not raised
     assert [vc._at(x) for x in (array, words, 5, None)] == got[:2] + got[3:]
+
+
+def test_documented_limits(vc):
+    """The sizes that the header gives are taken as far as the check for a GPU goes (which a machine
+    without one fails), and the next one is refused."""
+    def window(**kw):
+        a = dict(Q=A, K=A, V=A, O=A, B=1, Hq=1, Hkv=1, Nq=1, Nk=1, d=64, scale_log2=0.1, dtype=vc.Dtype.F16)
+        a.update(kw)
+        return vc.flash_window_fwd(**a)
+
+    def attn(heads=1, **kw):
+        a = dict(cache=vc.kv8_cache(A, A, A, A, 1, heads, 16, 64), Q=A, O=A, table=A, table_width=1, lens=A, B=1,
+                 Hq=heads, scale_log2=0.1, dtype=vc.Dtype.F16, workspace=A, workspace_bytes=0)
+        a.update(kw)
+        return vc.kv8_attn(**a)
+
+    refused = (INVALID,)
+    if vc.vcInit() == 0:
+        pytest.skip("with a GPU the host addresses are refused by themselves")
+    assert window(B=65535) not in refused and window(B=65536) in refused
+    assert window(Hq=65535) not in refused and window(Hq=32768, B=2) in refused
+    assert window(Nq=1 << 30) not in refused and window(Nq=(1 << 30) + 1) in refused
+    assert window(Nk=1 << 30) not in refused and window(Nk=(1 << 30) + 1) in refused
+    assert attn(B=65535) not in refused and attn(B=65536) in refused
+    assert attn(Hq=65535) not in refused and attn(Hq=65536) in refused
+    assert attn(heads=65535) not in refused and attn(heads=65536) in refused
+    most = ((1 << 31) - 1) // 16
+    assert attn(table_width=most) not in refused and attn(table_width=most + 1) in refused
