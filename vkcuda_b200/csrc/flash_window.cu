@@ -8,9 +8,10 @@
 // over j <= t with t - j < window or j < sinks, and j < lens[b].
 //
 // Bound: the tensor cores, 4 d operations per visible (row, key) pair.
-// Measured (bf16, 32 heads over 8 K/V heads of 128): 8192 tokens through a
-// window of 2048 246 us, 980 TFLOP/s of visible work; the last 2048 of 6144
-// through 4096 268 us, 1030 TFLOP/s (0.62 of the dense peak). A step of 128 keys
+// Measured (bf16, 32 heads over 8 K/V heads of 128, short runs at 1.9 GHz): 8192
+// tokens through a window of 2048 246 us, 980 TFLOP/s of visible work; the last
+// 2048 of 6144 through 4096 268 us, 1030 TFLOP/s (0.62 of the dense peak); on
+// another GPU 271 and 291 us. A step of 128 keys
 // for both row tiles takes ~3600 cycles, of which the MMAs are 2048; the issuing
 // warp spends ~2500 (75 to 80 cycles an MMA) and waits ~900 for P.
 //
@@ -812,8 +813,10 @@ cudaError_t launch_flash_window(const FlashWindowArgs &a, cudaStream_t stream) {
   // every row tile can have an SM of its own, two halves of its keys do: 8 heads
   // x 512 tokens 10.6 us (with one row tile a CTA, whose steps follow one another,
   // 11.4), x 1024 14.7 (17.6), x 2048 22.9 (29.4), 2 x 8192 of d 64 57.5 (85).
-  // With more row tiles than SMs it is the other way round (32 x 2048, 512 tiles:
-  // 57 us split, 51 in pairs), or the same (256 tiles: 35.5 and 35.8).
+  // With many more row tiles than SMs it is the other way round (32 x 2048, 512
+  // tiles: 57 us split, 51 in pairs; 256: 36.1 and 34.8). In between it depends on
+  // the window: 160 tiles 27.5 split, 34.4 in pairs without one, 19.1 and 17.5
+  // through 512 keys; 192 32.5 and 34.3; 224 34.9 and 34.4, 23.8 and 18.9.
   const bool split = units * p.slices <= sm_count_current();
   p.items = (int)(split ? units : (units + 1) / 2);
   const int grid = p.items * p.slices;

@@ -28,8 +28,9 @@
 // reads below meet no bank twice. Warps of a block meet only where an item
 // ends: there each joins a quarter of the results, while the next item's queries
 // are on their way (two warps, then one, and the queries after that: 256 sequences
-// of up to 500 tokens took 63.6 us instead of 55.0). Rows that the mask hides arrive too; their scores become minus
-// infinity and their values zero, whatever they hold. Per 16 keys, with
+// of up to 500 tokens took 63.6 us instead of 55.0; that is 57 on another GPU, and
+// 59 with the sum's own maximum). Rows that the mask hides arrive too; their scores
+// become minus infinity and their values zero, whatever they hold. Per 16 keys, with
 // m16n8k16 fp16 products and fp32 accumulators:
 //   S^T = K Q^T   A = the codes as fp16 (exact), rows keys; B = q. The order of
 //                 d within the product is free, so that a thread's operands are
