@@ -145,3 +145,115 @@ def test_window_same_answer_each_time(gpu, shape, t):
             torch.cuda.synchronize()
     _done(gpu)
     assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("Hq,H,d,n,P", [(8, 2, 64, 200, 16), (32, 8, 128, 700, 64)])
+def test_calls_that_follow_at_once_see_each_other(gpu, Hq, H, d, n, P, t):
+    """Launches overlap the one before them: prompt attention, append of its output, page copies,
+    attention over the copies, whose output is the next prompt's query, without a wait and with one
+    after each call; on the default stream, on another, and in a graph."""
+    pages = -(-n // P)
+    rng = np.random.default_rng(n)
+    ids = rng.permutation(2 * pages).astype(np.int32)
+    src, dst = _ints(ids[:pages]), _ints(ids[pages:])
+    x = [torch.randn(1, H, n, d, device="cuda").to(t) for _ in range(2)]
+    q0 = torch.randn(1, Hq, n, d, device="cuda").to(t)
+
+    def chain(rounds, after, stream=None):
+        s = stream if stream is not None else torch.cuda.default_stream()
+        with torch.cuda.stream(s):
+            c = Cache(gpu, 2 * pages, H, P, d)
+            q, o = q0.clone(), torch.zeros(1, Hq, n, d, device="cuda", dtype=t)
+            one = [torch.zeros(1, Hq, d, device="cuda", dtype=t) for _ in range(2)]
+            zero, lens = _ints([0]), _ints([0])
+            ws = torch.zeros(gpu.kv8_attn_workspace(c.handle, 1, Hq)[1], dtype=torch.uint8, device="cuda")
+            out = torch.zeros(rounds, 2, Hq, d, device="cuda", dtype=t)
+            torch.cuda.synchronize()
+
+            def go(i, s):
+                assert gpu.flash_window_fwd(q, x[0], x[1], o, 1, Hq, H, n, n, d, 0.2, _dt(gpu, t), window=90, sinks=2,
+                                            stream=s) == 0
+                after()
+                # The output's memory as tokens of the cache, V one row on.
+                assert gpu.kv8_append(c.handle, o, o[:, :, 1:], n - 1, src.view(1, -1), pages, zero, 1, n - 1, _dt(gpu, t),
+                                      lens_out=lens, k_stride=H * d, v_stride=H * d, stream=s) == 0
+                after()
+                assert gpu.kv8_copy_pages(gpu.kv8_layers([c.handle]), src, dst, pages, stream=s) == 0
+                after()
+                # Hq rows of the first head as queries, from row 0 and from row 1 on.
+                for side, (table, to) in enumerate(((dst, one[0]), (src, one[1]))):
+                    assert gpu.kv8_attn(c.handle, q[0, :, side], to, table.view(1, -1), pages, lens, 1, Hq, 0.2,
+                                        _dt(gpu, t), ws, ws.numel(), window=60, sinks=1, stream=s) == 0
+                    after()
+            return c, q, one, out, go, s
+
+    def run(rounds, after, stream=None):
+        c, q, one, out, go, s = chain(rounds, after, stream)
+        with torch.cuda.stream(s):
+            for i in range(rounds):
+                go(i, s)
+                out[i, 0].copy_(one[0][0])
+                out[i, 1].copy_(one[1][0])
+                q[0, :, :2].copy_(torch.stack(one)[:, 0].transpose(0, 1))
+        torch.cuda.synchronize()
+        return out
+
+    rounds = 40
+    want = run(rounds, torch.cuda.synchronize)
+    assert torch.isfinite(want).all() and want.abs().max() > 0.01
+    assert not torch.equal(want[:, 0], want[:, 1])
+    for stream in (None, torch.cuda.Stream()):
+        assert torch.equal(run(rounds, lambda: None, stream), want)
+    c, q, one, out, go, _ = chain(rounds, lambda: None)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go(0, torch.cuda.current_stream())
+        q[0, :, :2].copy_(torch.stack(one)[:, 0].transpose(0, 1))
+    for i in range(rounds):
+        graph.replay()
+        out[i, 0].copy_(one[0][0])
+        out[i, 1].copy_(one[1][0])
+    _done(gpu)
+    assert torch.equal(out, want)
+
+
+def test_two_threads_at_once(gpu):
+    """Calls of two host threads, each with a stream, a workspace and outputs of its own, over one
+    cache: what one thread alone gets."""
+    import threading
+    rng = np.random.default_rng(41)
+    lens = [900, 17, 300]
+    c, table = _fill(gpu, lens, 2, 32, 128, rng)
+    tab, ln = _ints(table), _ints(lens)
+    q = torch.randn(3, 8, 128, device="cuda").half()
+    p = torch.randn(1, 8, 500, 128, device="cuda").half()
+    need = gpu.kv8_attn_workspace(c.handle, 3, 8)[1]
+    torch.cuda.synchronize()
+    results, errors = {}, []
+
+    def work(name, count):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+            o = [torch.zeros_like(q) for _ in range(count)]
+            w = [torch.zeros_like(p) for _ in range(count)]
+        for i in range(count):
+            errors.append(int(gpu.kv8_attn(c.handle, q, o[i], tab, table.shape[1], ln, 3, 8, 0.12, gpu.Dtype.F16, ws,
+                                           need, stream=s)))
+            errors.append(int(gpu.flash_window_fwd(p, p, p, w[i], 1, 8, 8, 500, 500, 128, 0.1, gpu.Dtype.F16,
+                                                   window=100, stream=s)))
+        s.synchronize()
+        results[name] = o, w
+
+    work("alone", 1)
+    threads = [threading.Thread(target=work, args=(i, 60)) for i in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    _done(gpu)
+    assert set(errors) == {0}
+    (o,), (w,) = results["alone"]
+    for i in range(2):
+        assert all(torch.equal(x, o) for x in results[i][0]) and all(torch.equal(x, w) for x in results[i][1])
