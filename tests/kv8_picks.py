@@ -59,3 +59,24 @@ def one_of_each_tile(rng, visible, tile=128):
         own = np.flatnonzero(visible[t * tile:(t + 1) * tile]) + t * tile
         out.append(own[0] if i % 3 == 0 else own[-1] if i % 3 == 1 or t == tiles[-1] else rng.choice(own))
     return np.array(out)
+
+
+def mixed(q, k, v, v_scale, scale_log2, u_out):
+    """Attention rows q [h][d] over k, v [n][d] (v with its pages' scales v_scale [n] in it), and a bound
+    from the weights as they are: the output's rounding; each weight times scale to fp16, 2^-11 of it
+    or 2^-25 of the largest; the scores' fp32 error (d + 8) 2^-24 of the sum of |q k|, in numerator and
+    sum; fp32 sums of up to 64 terms in a row and exponentials, 2^-17."""
+    out, tol = [], []
+    d = q.shape[1]
+    for x in q:
+        s = (k @ x) * scale_log2
+        p = np.exp2(s - s.max())
+        p /= p.sum()
+        w = p * v_scale
+        code = np.abs(v) / np.where(v_scale > 0, v_scale, 1.0)[:, None]
+        o = p @ v
+        ds = (d + 8) * 2.0 ** -24 * (np.abs(k) @ np.abs(x)).max() * scale_log2
+        out.append(o)
+        tol.append(u_out * np.abs(o) + np.maximum(w * 2.0 ** -11, w.max() * 2.0 ** -25) @ code +
+                   (2 * np.log(2) * ds + 2.0 ** -17) * (p @ np.abs(v)) + 2.0 ** -24)
+    return np.stack(out), np.stack(tol)

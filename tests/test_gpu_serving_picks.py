@@ -126,3 +126,33 @@ def test_window_every_tile_counts(gpu, Nq, Nk, Hq, d, window, sinks, t):
         for x, (h, i) in enumerate(ask):
             off = np.abs(got[h, i] - expect[i].want(pos[x:x + 1])) - expect[i].bound(pos[x:x + 1])
             assert (off <= 0).all(), (h, i, pos[x], off.max())
+
+
+@pytest.mark.parametrize("t", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("n,G,d,window", [(3000, 4, 128, 0), (20011, 8, 64, 0), (300001, 16, 64, 0),
+                                          (300001, 4, 64, 200000)])
+def test_attn_mixed_values_of_long_sequences(gpu, n, G, d, window, t):
+    """Random keys and values, compared within a bound from the actual weights."""
+    P = 64
+    rng = np.random.default_rng(n + G)
+    pages = -(-n // P)
+    c = Cache(gpu, pages, 1, P, d)
+    for codes, scales in ((c.k, c.ks), (c.v, c.vs)):
+        codes.copy_((torch.randn(codes.shape, device="cuda") * 100).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8))
+        scales.copy_(torch.from_numpy(rng.uniform(0.5, 2, (pages, 1)).astype(np.float32)) * 2.0 ** -7)
+    table = rng.permutation(pages).astype(np.int32)[None]
+    q = torch.randn(1, G, d, device="cuda").to(t)
+    o = torch.full_like(q, 7.0)
+    ws = torch.zeros(gpu.kv8_attn_workspace(c.handle, 1, G)[1], dtype=torch.uint8, device="cuda")
+    scale = 1.4426950408889634 / d ** 0.5
+    assert gpu.kv8_attn(c.handle, q, o, _ints(table), pages, _ints([n]), 1, G, scale, _dt(gpu, t), ws, ws.numel(),
+                        window=window, sinks=4) == 0
+    _done(gpu)
+    seen = plain.visible(n - 1, n, window, 4)
+    page, slot = table[0][seen // P], seen % P
+    kc, ks, vc, vs = c.host()
+    k = plain.E4M3[kc[page, 0, slot]] * ks[page, 0].astype(np.float64)[:, None]
+    v = plain.E4M3[vc[page, 0, slot]] * vs[page, 0].astype(np.float64)[:, None]
+    want, tol = picks.mixed(_f64(q)[0], k, v, vs[page, 0].astype(np.float64), scale, torch.finfo(t).eps / 2)
+    off = np.abs(_f64(o)[0] - want) - tol
+    assert (off <= 0).all(), (off.max(), tol.min(), np.abs(want).max())

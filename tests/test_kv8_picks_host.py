@@ -43,3 +43,20 @@ def test_wrong_results_are_rejected(n, window, sinks, u_out, u_weight):
     keep[tiles[len(tiles) // 4] * 128:] = False
     assert not passes(result(keep))[pos >= tiles[len(tiles) // 4] * 128].any()
     assert not passes(result(visible) * 2).any()
+
+
+@pytest.mark.parametrize("n,u_out", [(20000, 2.0 ** -11), (300000, 2.0 ** -8)])
+def test_mixed_results_without_a_part_are_rejected(n, u_out):
+    """Random data, whose outputs shrink with the root of the keys: the bound from the actual weights
+    still tells zeros, half of the keys and a lost eighth from the result."""
+    rng, d = np.random.default_rng(n), 64
+    q, k, v = rng.standard_normal((3, d)), rng.standard_normal((n, d)), rng.standard_normal((n, d))
+    scale = 1.4426950408889634 / 8
+    want, tol = picks.mixed(q, k, v, np.ones(n), scale, u_out)
+    assert all(np.abs(plain._row(x, k, v, scale) - w).max() < 1e-12 for x, w in zip(q, want))
+    for lost in (slice(0, n), slice(n // 2, n), slice(n // 4, n // 4 + n // 8)):
+        keep = np.ones(n, bool)
+        keep[lost] = False
+        for x, w, t in zip(q, want, tol):
+            got = plain._row(x, k[keep], v[keep], scale)
+            assert not (np.abs(got - w) <= t).all(), lost

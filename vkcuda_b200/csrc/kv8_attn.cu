@@ -66,7 +66,7 @@ constexpr int kTile = 128;     // keys per tile
 constexpr int kWarps = 4;      // 32 keys each
 constexpr int kThreads = kWarps * 32;
 // Two blocks with 16 KB of ring per warp: 32 sequences of up to 16384 tokens
-// 105 us, one of 32000 17.6 us, 64 of up to 700 25.4 us (104, 19 and 23.0 since).
+// 105 us, one of 32000 17.6 us, 64 of up to 700 25.4 us (104, 19 and 23 to 25 since).
 // Three: 109, 20.6 (more parts to join) and 23.3 us; one block of 8 warps: 109,
 // 14.5 and 31.8 us.
 constexpr int kBlocksPerSm = 2;

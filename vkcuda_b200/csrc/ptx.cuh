@@ -740,7 +740,7 @@ __device__ __forceinline__ float ex2_approx(float x) {
   }                                                                       \
   void *fname##_word() {                                                  \
     void *at = nullptr;                                                   \
-    return cudaGetSymbolAddress(&at, vc_dev_error) == cudaSuccess ? at    \
-                                                                  : nullptr; \
+    const cudaError_t e = cudaGetSymbolAddress(&at, vc_dev_error);        \
+    return e == cudaSuccess ? at : nullptr;                               \
   }                                                                       \
   }
